@@ -243,6 +243,73 @@ int tvk_embedding(const void* table, const int32_t* tokens, void* out, int n_tok
 int tvk_argmax(const void* logits, int32_t* out, int rows, int vocab, long long row_stride, int dtype,
                void* stream);
 
+/* ------------------------------------------------------------------------
+ * The 8-bit K/V cache (no counterpart in the reference).  k_cache / v_cache hold
+ * e4m3 codes [num_blocks, block_size, n_kv_heads, head_dim] (one layer), k_scale /
+ * v_scale one fp32 scale per block and KV head [num_blocks, n_kv_heads]; a value
+ * is code * scale.  Zeroed codes and scales are an empty cache.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * K/V rows [n_tokens, n_kv_heads, head_dim] (dtype) -> 8-bit slots, the
+ * counterpart of tvk_write_kv_slots.  Slots are flat (block * block_size +
+ * offset); negative and out-of-pool slots are skipped; of several rows for one
+ * slot the last counts.  For each (block, head) that rows land in, K and V apart:
+ *   old = 0 if the call writes the block's offset 0 (the block starts anew: its
+ *         other rows become zeros), else its scale (0 if not positive and finite)
+ *   now = max(old, 2^k), k >= -100 the smallest with amax <= 448 * 2^k over the
+ *         finite values of those rows
+ *   the call's rows become e4m3(x / now) (nearest-even; non-finite values NaN), the
+ *   block's other rows e4m3(code * (old / now)), the scale now.
+ * So a sequence's blocks are filled from offset 0 on, in any number of calls.
+ * A call's result does not depend on the order its blocks are worked in.
+ * head_dim a multiple of 16, block_size <= 1024; k, v and the caches 16-byte aligned.
+ */
+int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t* slots, void* k_cache, void* v_cache,
+                          float* k_scale, float* v_scale, int n_tokens, int n_kv_heads, int head_dim,
+                          int num_blocks, int block_size, int dtype, void* stream);
+
+/*
+ * Bytes of scratch tvk_paged_decode_attention_q8 needs: a 256-byte header (the
+ * status word at byte 0), a fixed area for the partial sums of sequences that
+ * several CTAs share, and one arrival counter per (sequence, KV head).  Zero all
+ * of it once; every call leaves header and counters zero (the status word only if
+ * no kernel wait timed out).  One workspace serves one stream at a time and is
+ * not shared with other entry points.
+ */
+size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads);
+
+/*
+ * tvk_paged_decode_attention over an 8-bit cache: the same arguments and masking
+ * (contexts, tables, max_context_len, zeros for an empty context, out-of-pool
+ * block ids read as zeros), with
+ *   out[b,0,h,:] = sum_t softmax_t(q[b,h] . K_t / sqrt(head_dim)) V_t,
+ *   K_t = k_scale[blk, h/g] * k_cache[blk, off, h/g], V_t likewise.
+ * q and out are fp32, fp16 or bf16; head_dim 32, 64 or 128; at most 16 query heads
+ * per KV head; any block size.  What lies behind a sequence's context is never
+ * used, whatever it holds.  q, k_cache and v_cache 16-byte aligned.
+ */
+int tvk_paged_decode_attention_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                  const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,
+                                  void* out, int batch, int n_heads, int n_kv_heads, int head_dim, int block_size,
+                                  int num_blocks, int max_blocks, int max_context_len, int dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of one token per row of logits [rows, vocab] (row stride in
+ * elements, any alignment of the element type), beside tvk_argmax; no counterpart in the
+ * reference.  With lse = log sum_v exp(logits[r, v]) in fp32:
+ *   logprobs[r]  = logits[r, tokens[r]] - lse; -inf for a token outside [0, vocab)
+ *   entropy[r]   = -sum_v p_v log p_v, p_v = exp(logits[r, v] - lse), 0 log 0 = 0
+ *   top_tokens / top_logprobs [rows, top_k]: the top_k most likely tokens and their
+ *                log probabilities, equal logits in index order; 0 <= top_k <= 32
+ * A row holding NaN or +inf, or nothing but -inf, has NaN log probabilities and
+ * entropy; its top tokens still go by the logits, NaN before everything.
+ */
+int tvk_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs, float* entropy,
+                       float* top_logprobs, int32_t* top_tokens, int rows, int vocab, long long row_stride, int top_k,
+                       int dtype, void* stream);
+
 /*
  * Paged-decode attention that allocates nothing (no counterpart in the
  * reference, which lets tinygrad allocate its temporaries).

@@ -52,6 +52,10 @@ SIGNATURES = {
     ),
     "tvk_probe_mma_issue": (_c_int, [_c_int, _c_int, _c_void, _c_int, _c_void]),
     "tvk_probe_exp_unit": (_c_int, [_c_int, _c_int, _c_void, _c_int, _c_void, _c_void]),
+    "tvk_write_kv_slots_q8": (_c_int, [_c_void] * 7 + [_c_int] * 6 + [_c_void]),
+    "tvk_paged_decode_q8_workspace_size": (_c_size, [_c_int] * 2),
+    "tvk_paged_decode_attention_q8": (_c_int, [_c_void] * 8 + [_c_int] * 9 + [_c_void, _c_size, _c_void]),
+    "tvk_token_logprobs": (_c_int, [_c_void] * 6 + [_c_int, _c_int, _c_int64, _c_int, _c_int, _c_void]),
 }
 
 _lib = None
@@ -113,3 +117,12 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
         elif t.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     return dev
+
+
+def call_on(dev: torch.device, fn, *args) -> int:
+    """``fn(*args)`` with ``dev`` as the current device (launches go to the current
+    device's context, and the tensors may live on another one)."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)

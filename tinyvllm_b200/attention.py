@@ -110,6 +110,61 @@ def paged_decode_attention(queries: torch.Tensor, k_cache: torch.Tensor, v_cache
     return out
 
 
+def paged_decode_attention_q8(queries: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                              k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                              context_lens: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                              block_size: int, max_context_len: Optional[int] = None, *,
+                              out: Optional[torch.Tensor] = None, check: bool = False) -> torch.Tensor:
+    """``paged_decode_attention`` over a cache held in 8 bits.
+
+    k_cache/v_cache ``torch.float8_e4m3fn`` codes [N,block_size,Hkv,D], k_scale/v_scale
+    fp32 [N,Hkv], one scale per block and KV head (``layers.write_kv_slots_q8`` fills
+    them; a value is code * scale).  queries [B,1,Hq,D] in fp32, fp16 or bf16;
+    everything else, and the masking, as in ``paged_decode_attention``.  Returns
+    [B,1,Hq,D] in the dtype of the queries.
+    """
+    dev = _lib.require_cuda(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+    B = queries.shape[0]
+    if queries.shape[1:] != (1, n_heads, head_dim):
+        raise ValueError(f"queries must be [B,1,{n_heads},{head_dim}], got {tuple(queries.shape)}")
+    if k_cache.dim() != 4 or k_cache.shape[1:] != (block_size, n_kv_heads, head_dim) or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache/v_cache must be [N,{block_size},{n_kv_heads},{head_dim}], got "
+                         f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
+    num_blocks = k_cache.shape[0]
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError("k_cache and v_cache must be float8_e4m3fn")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("k_scale and v_scale must be float32")
+    if k_scale.shape != (num_blocks, n_kv_heads) or v_scale.shape != k_scale.shape:
+        raise ValueError(f"k_scale/v_scale must be [{num_blocks},{n_kv_heads}], got {tuple(k_scale.shape)} / "
+                         f"{tuple(v_scale.shape)}")
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise TypeError("block_tables and context_lens must be int32")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or context_lens.shape != (B,):
+        raise ValueError("block_tables must be [B,max_blocks] and context_lens [B]")
+    if not (queries.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_scale.is_contiguous() and v_scale.is_contiguous() and block_tables.is_contiguous()
+            and context_lens.is_contiguous()):
+        raise ValueError("all tensors must be contiguous")
+    if out is None:
+        out = torch.empty_like(queries)
+    elif (out.shape != queries.shape or out.dtype != queries.dtype or out.device != dev
+          or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor like queries")
+    L = _lib.lib()
+    ws = _workspace(dev, L.tvk_paged_decode_q8_workspace_size(B, n_kv_heads), "decode_q8")
+    rc = _lib.call_on(
+        dev, L.tvk_paged_decode_attention_q8, queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
+        B, n_heads, n_kv_heads, head_dim, block_size, num_blocks, block_tables.shape[1],
+        -1 if max_context_len is None else int(max_context_len), _lib.dtype_code(queries), ws.data_ptr(), ws.numel(),
+        _lib.stream_ptr(dev))
+    _lib.check(rc, "tvk_paged_decode_attention_q8")
+    if check:
+        check_workspace(dev, "decode_q8", "tvk_paged_decode_attention_q8")
+    return out
+
+
 def flash_prefill_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                    cu_seqlens: torch.Tensor, max_seqlen: int, causal: bool = True, *,
                                    slot_mapping: Optional[torch.Tensor] = None,

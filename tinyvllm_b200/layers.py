@@ -7,7 +7,7 @@ fp32 with one rounding to the storage dtype.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -135,6 +135,39 @@ def write_kv_slots(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cach
     _lib.check(rc, "tvk_write_kv_slots")
 
 
+def write_kv_slots_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """``write_kv_slots`` into an 8-bit cache: k/v [T,Hkv,D] (fp32, fp16 or bf16) -> e4m3
+    codes [N,block_size,Hkv,D] with one fp32 scale per block and head [N,Hkv], in place.
+
+    A call that writes a block's offset 0 starts the block anew; otherwise the block
+    keeps its rows, and its scale grows where the new rows need it (to a power of two,
+    so the rows already there change their exponents only).  Rows with negative or
+    out-of-pool slots are skipped; of several rows for one slot the last counts;
+    values that are not finite are stored as NaN."""
+    dev = _lib.require_cuda(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    _contig(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k/v must be [T,Hkv,D] and the caches [N,block_size,Hkv,D], got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    T, hkv, d = k.shape
+    nb, bs = k_cache.shape[:2]
+    if k_cache.shape[2:] != (hkv, d) or k_scale.shape != (nb, hkv) or v_scale.shape != (nb, hkv):
+        raise ValueError(f"caches must be [N,block_size,{hkv},{d}] with scales [N,{hkv}]")
+    if v.dtype != k.dtype:
+        raise TypeError("k and v must share one dtype")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError("k_cache and v_cache must be float8_e4m3fn")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("k_scale and v_scale must be float32")
+    if slots.dtype != torch.int64 or slots.shape != (T,):
+        raise TypeError("slots must be int64 [T]")
+    rc = _lib.call_on(dev, _lib.lib().tvk_write_kv_slots_q8, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
+                      k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, hkv, d, nb, bs,
+                      _lib.dtype_code(k), _stream(dev))
+    _lib.check(rc, "tvk_write_kv_slots_q8")
+
+
 def silu_mul(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """silu(a) * b over the last dim (llama.py:221); a/b may be column slices of one
     packed [rows, 2H] gate|up tensor."""
@@ -181,3 +214,42 @@ def greedy_argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> t
                                _stream(dev))
     _lib.check(rc, "tvk_argmax")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns, one row per row of logits."""
+    logprobs: torch.Tensor       # fp32 [R]
+    entropy: torch.Tensor        # fp32 [R], in nats
+    top_logprobs: torch.Tensor   # fp32 [R, K]
+    top_tokens: torch.Tensor     # int32 [R, K]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens[r]`` (int32 [R]) under ``softmax(logits[r])``, that
+    distribution's entropy and its ``top_k`` (0 to 32) most likely tokens, in one pass
+    over the logits [R, V] (rows may be strided).  Arithmetic is fp32.
+
+    Equal logits rank in index order.  A token outside the vocabulary has -inf; a row
+    with NaN or +inf, or with nothing but -inf, has NaN values."""
+    dev = _lib.require_cuda(logits, tokens)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [R, V] with contiguous rows")
+    rows, vocab = logits.shape
+    if not 0 <= top_k <= min(32, vocab):
+        raise ValueError(f"top_k must be in [0, min(32, {vocab})], got {top_k}")
+    if tokens.dtype != torch.int32 or tokens.shape != (rows,):
+        raise TypeError("tokens must be int32 [R]")
+    if not tokens.is_contiguous():
+        raise ValueError("tensors must be contiguous")
+    row_stride = logits.stride(0) if rows > 1 else vocab
+    if row_stride < vocab:
+        raise ValueError("rows of logits must not overlap")
+    # one allocation for the three fp32 results, the tokens apart
+    f = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=dev)
+    lp, ent, top = f[:rows], f[rows:2 * rows], f[2 * rows:].view(rows, top_k)
+    top_tokens = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+    rc = _lib.call_on(dev, _lib.lib().tvk_token_logprobs, logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(),
+                      ent.data_ptr(), top.data_ptr(), top_tokens.data_ptr(), rows, vocab, row_stride, top_k,
+                      _lib.dtype_code(logits), _stream(dev))
+    _lib.check(rc, "tvk_token_logprobs")
+    return TokenLogprobs(lp, ent, top, top_tokens)
