@@ -18,6 +18,9 @@
 // not depend on who that is.  Nobody waits for anybody.
 #include <math.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "kv_cache_q8.cuh"
 
 namespace {
@@ -26,6 +29,7 @@ constexpr int kTile = 64;            // tokens per tile of the work line
 constexpr int kSimtTile = 32;        // tokens the simt kernel stages at a time
 constexpr int kMaxGroup = 16;        // query heads per KV head
 constexpr int kMaxCtas = 592;        // pieces a call is cut into at most (four CTAs on each of 148 SMs)
+constexpr int kTcCtas = 296;         // the same for the tensor-core kernel: two CTAs on each SM
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
 constexpr int kMinPiece = 4;         // shortest piece, in tiles
 constexpr int kSlotFloats = 2240;    // partials of one cut unit: rows * (D + 2), at most 64 * 34, 32 * 66 or 16 * 130
@@ -42,7 +46,10 @@ struct Q8Params {
   int* counters;   // [batch * n_kv_heads], zero between calls
   int batch, n_heads, n_kv_heads, group, block_size, num_blocks, max_blocks;
   int max_ctx_tokens;
-  float scale_log2;  // log2(e) / sqrt(head_dim)
+  float scale_log2;            // log2(e) / sqrt(head_dim)
+  int n_stages;                // ring depth of the tensor-core kernel
+  unsigned long long wait_ns;  // wall-time limit of every mbarrier wait
+  int drop_loads;              // wait-limit test: the producer issues nothing, so waits run out
 };
 
 __device__ __forceinline__ int effective_ctx(const Q8Params& p, int b) {
@@ -147,25 +154,12 @@ __device__ __forceinline__ float* part_slot(const Q8Params& p, int cta, bool is_
   return p.part + (size_t)(cta * 2 + (is_first ? 1 : 0)) * kSlotFloats;
 }
 
-// The end of a share, by the NT threads that hold it: `m`, `l` [rows] and `o`
-// [rows][D] in shared memory (o unnormalised, relative to m), rows = query heads
-// from row0 on of sequence s.b.  Writes the output rows, or the partials, or as the
-// last to arrive the sum of all partials.  `flag` is a shared int; `sync` a
-// barrier of the NT threads.
+// The end of a cut unit's share, by the NT threads that have just stored its
+// partials with __stcg (o [rows][D], then m, l [rows][2]): counts the arrival, and
+// the last to arrive adds the parts up and writes the output rows (query heads from
+// row0 on).  `flag` is a shared int; `sync` a barrier of the NT threads.
 template <typename T, int D, int NT, typename Sync>
-__device__ void finish_share(const Q8Params& p, const Share& s, int unit, int rows, int row0, const float* m,
-                             const float* l, const float* o, int* flag, int tid, Sync sync) {
-  T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + row0) * D;
-  if (s.n_parts == 1) {
-    for (int i = tid; i < rows * D; i += NT) out[i] = DT<T>::from_f(o[i] / l[i / D]);
-    return;
-  }
-  float* mine = part_slot(p, blockIdx.x, (int)blockIdx.x == s.first_cta);
-  for (int i = tid; i < rows * D; i += NT) __stcg(mine + i, o[i]);
-  for (int i = tid; i < rows; i += NT) {
-    __stcg(mine + rows * D + i * 2, m[i]);
-    __stcg(mine + rows * D + i * 2 + 1, l[i]);
-  }
+__device__ void join_parts(const Q8Params& p, const Share& s, int unit, int rows, int row0, int* flag, int tid, Sync sync) {
   __threadfence();
   sync();
   if (tid == 0) {
@@ -176,6 +170,7 @@ __device__ void finish_share(const Q8Params& p, const Share& s, int unit, int ro
   }
   sync();
   if (!*flag) return;
+  T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + row0) * D;
   for (int i = tid; i < rows * D; i += NT) {
     const int r = i / D;
     float M = -INFINITY;
@@ -313,7 +308,454 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
       if (idx < G * D) qs[idx] = acc[k];
     }
     __syncthreads();
-    finish_share<T, D, 128>(p, s, s.b * Hkv + s.h, G, s.h * G, mfin, lfin, qs, &flag, tid, [] { __syncthreads(); });
+    if (s.n_parts == 1) {
+      for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(qs[i] / lfin[i / D]);
+      continue;
+    }
+    float* mine = part_slot(p, blockIdx.x, (int)blockIdx.x == s.first_cta);
+    for (int i = tid; i < G * D; i += 128) __stcg(mine + i, qs[i]);
+    for (int i = tid; i < G; i += 128) {
+      __stcg(mine + G * D + i * 2, mfin[i]);
+      __stcg(mine + G * D + i * 2 + 1, lfin[i]);
+    }
+    join_parts<T, D, 128>(p, s, s.b * Hkv + s.h, G, s.h * G, &flag, tid, [] { __syncthreads(); });
+  }
+}
+
+// -----------------------------------------------------------------------------
+// Tensor-core kernel: 16-bit queries; block sizes 8, 16, 32 and multiples of 64.
+//
+// A unit is HP neighbouring KV heads of one sequence (HP * D bytes a token, 128
+// where the head count allows), so that one TMA row is a whole 128-byte line also
+// for small heads.  One producer warp streams 64-token tiles of codes (and their
+// scales, by 4-byte asynchronous copies, and at a share's start its query rows)
+// through a ring of stages; four consumer warps take 16 tokens of a tile each:
+//   S^T [16 tokens, 8 heads] = K . Q^T    A = codes as halves, straight from their rows
+//   P^T                       = 2^(S^T - m) as halves, transposed in registers
+//   O^T [D, 8 heads]         += v_scale * (V^T . P^T)
+// Tokens and dims, not heads, are the 16-row side of the products: at 4 to 8
+// query heads per KV head that halves the matrix instructions and the accumulators.
+// The order of the k index of a product is free, so a lane takes 16 neighbouring
+// bytes of its row as four k steps and nothing is shuffled; for V a byte
+// permute pairs the same dim of two tokens.
+// -----------------------------------------------------------------------------
+template <int ROWB>
+__device__ __forceinline__ uint32_t row_off(int t, int byte) {  // as the TMA swizzle of ROWB-byte rows lays it
+  const int x = ROWB == 128 ? (t & 7) : ROWB == 64 ? ((t >> 1) & 3) : ((t >> 2) & 1);
+  return t * ROWB + ((((byte >> 4) ^ x) << 4) | (byte & 15));
+}
+
+constexpr int kTcThreads = 160;
+constexpr int kScaleFloats = 64;  // scales per stage: K and V, HP <= 4 heads, <= 8 blocks
+
+template <int D, int HP>
+struct TcLayout {
+  static constexpr int ROWB = D * HP;
+  static constexpr int kPart = kTile * ROWB;  // K (or V) codes of a stage
+  // stage = K codes, V codes, scales, query rows
+  static __host__ __device__ int q_bytes(int group) { return HP * group * D * 2; }
+  static __host__ __device__ int scales_off(int n_stages) { return n_stages * 2 * kPart; }
+  static __host__ __device__ int q_off(int n_stages) { return scales_off(n_stages) + n_stages * kScaleFloats * 4; }
+  static __host__ __device__ int merge_off(int n_stages, int group) { return q_off(n_stages) + n_stages * q_bytes(group); }
+  // merge: o [4][HP * group][D], m, l and weights [4][HP * group], one flag
+  static __host__ __device__ int bar_off(int n_stages, int group) {
+    return merge_off(n_stages, group) + 4 * HP * group * (D + 3) * 4 + 16;
+  }
+  static __host__ __device__ int bytes(int n_stages, int group) { return bar_off(n_stages, group) + n_stages * 16 + 1024; }
+};
+
+template <typename T, int D, int HP, int NT, bool BS8>
+__global__ void __launch_bounds__(kTcThreads, 2)
+    paged_decode_q8_tc_kernel(const Q8Params p, const __grid_constant__ CUtensorMap tm_k,
+                              const __grid_constant__ CUtensorMap tm_v) {
+  using L = TcLayout<D, HP>;
+  constexpr int ROWB = L::ROWB;
+  constexpr int KS = D / 16;  // k steps of S, and 16-dim tiles of O
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base_u32 = (raw + 1023u) & ~1023u;
+  uint8_t* base = smem_raw + (base_u32 - raw);
+  const int G = p.group, NS = p.n_stages;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(base + ((L::bar_off(NS, G) + 7) & ~7));
+  uint64_t* empty_bar = full_bar + NS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(&full_bar[s], 33);  // the byte count, and every producer lane's scales
+      ptx::mbar_init(&empty_bar[s], 4);
+    }
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int heads = p.n_kv_heads / HP;
+  Walker w;
+  w.start(p, heads, lane);
+  Share s;
+  int stage = 0;
+  uint32_t phase = 0;
+
+  if (warp == 4) {
+    // ---------------- producer ----------------
+    if (lane == 0) {
+      ptx::prefetch_tmap(&tm_k);
+      ptx::prefetch_tmap(&tm_v);
+    }
+    const int rows = p.block_size < kTile ? p.block_size : kTile;  // rows of one TMA box
+    const int nb = kTile / rows;                                   // blocks of a tile
+    const int q_bytes = L::q_bytes(G);
+    bool running = true;
+    while (running && w.next(p, s)) {
+      const int32_t* bt = p.block_tables + (size_t)s.b * p.max_blocks;
+      const int blk_end = (s.tok1 + p.block_size - 1) / p.block_size;
+      constexpr int W = 4;  // ids of 128 blocks at a time, one per lane and register
+      int win = -W * 32, id[W];
+      for (int t0 = s.tok0; t0 < s.tok1; t0 += kTile) {
+        const int first = t0 / p.block_size;
+        if (first + nb > win + W * 32) {
+          win = first;
+#pragma unroll
+          for (int r = 0; r < W; ++r) {
+            const int i = win + r * 32 + lane;
+            id[r] = i < blk_end ? __ldg(bt + i) : -1;
+          }
+        }
+        if (!ptx::mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_ns)) {
+          if (lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+          running = false;
+          break;
+        }
+        if (!p.drop_loads) {
+          const int live = min(nb, blk_end - first);
+          if (lane == 0) {
+            uint32_t tx = (uint32_t)(live * rows * ROWB * 2);
+            if (t0 == s.tok0) tx += q_bytes;
+            ptx::mbar_arrive_expect_tx(&full_bar[stage], tx);
+            if (t0 == s.tok0)
+              ptx::bulk_load(base + L::q_off(NS) + stage * q_bytes,
+                             reinterpret_cast<const uint8_t*>(p.q) + ((size_t)s.b * p.n_heads + (size_t)s.h * HP * G) * D * 2,
+                             (uint32_t)q_bytes, &full_bar[stage]);
+          }
+          __syncwarp();
+          // lane = block of the tile (up to 8) and, for the scales, head and K / V
+          const uint32_t codes = base_u32 + stage * 2 * L::kPart;
+          const uint32_t scales = base_u32 + L::scales_off(NS) + stage * kScaleFloats * 4;
+          for (int i0 = 0; i0 < nb * 2 * HP; i0 += 32) {
+            const int i = i0 + lane, j = i % nb, kv = (i / nb) & 1, hp = i / (2 * nb);
+            const int rel = first + j - win;
+            int blk = -1;
+#pragma unroll
+            for (int r = 0; r < W; ++r) {
+              const int v = __shfl_sync(0xffffffffu, id[r], rel & 31);
+              blk = (rel >> 5) == r ? v : blk;
+            }
+            if (i < nb * 2 * HP) {
+              const bool in = j < live && blk >= 0 && blk < p.num_blocks;
+              const float* src = kv ? p.v_scale : p.k_scale;
+              q8::copy4_async(scales + ((kv * HP + hp) * nb + j) * 4,
+                              in ? src + (size_t)blk * p.n_kv_heads + s.h * HP + hp : src, in);
+              if (hp == 0 && j < live)
+                q8::tma_load_3d(codes + kv * L::kPart + j * rows * ROWB, kv ? &tm_v : &tm_k, &full_bar[stage],
+                                s.h * HP * D, t0 % p.block_size, blk);
+            }
+          }
+          q8::arrive_after_copies(&full_bar[stage]);
+        }
+        if (++stage == NS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // No copy is in flight when the CTA ends, whatever became of the consumers.
+    for (int i = 0; i < NS && !p.drop_loads; ++i) {
+      if (!ptx::mbar_wait(&full_bar[stage], phase ^ 1, p.wait_ns)) break;
+      if (++stage == NS) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int g = lane >> 2, tig = lane & 3;
+  const int nb = p.block_size < kTile ? kTile / p.block_size : 1;
+  const int R = HP * G;  // output rows of a unit
+  float* co = reinterpret_cast<float*>(base + L::merge_off(NS, G));
+  float* cm = co + 4 * R * D;
+  float* cl = cm + 4 * R;
+  float* cw = cl + 4 * R;
+  int* flag = reinterpret_cast<int*>(cw + 4 * R);
+  // Row r of an 8-token group is token tok_of(r): an order in which the lanes of one
+  // shared-memory access fall on different banks.
+  auto tok_of = [](int r) { return HP == 1 ? r : HP == 2 ? (r >> 1) | ((r & 1) << 2) : ((r & 3) << 1) | (r >> 2); };
+  const int tk = tok_of(g), tv0 = tok_of(2 * tig), tv1 = tok_of(2 * tig + 1);
+  bool dead = false;  // a wait ran out: go through the motions, so that every counter is met
+
+  while (w.next(p, s)) {
+    if (s.ctx == 0) {
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * R) * D;
+      for (int i = threadIdx.x; i < R * D; i += 128) out[i] = DT<T>::from_f(0.f);
+      continue;
+    }
+    uint32_t qb[HP][NT][KS][2];
+    float o[HP][NT][KS][4], m[HP][NT][2], l[HP][NT][2], hs[HP][NT][2];
+#pragma unroll
+    for (int hp = 0; hp < HP; ++hp)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[hp][n][i][0] = o[hp][n][i][1] = o[hp][n][i][2] = o[hp][n][i][3] = 0.f;
+          qb[hp][n][i][0] = qb[hp][n][i][1] = 0u;
+        }
+        m[hp][n][0] = m[hp][n][1] = -INFINITY;
+        l[hp][n][0] = l[hp][n][1] = 0.f;
+        hs[hp][n][0] = hs[hp][n][1] = p.scale_log2;
+      }
+    for (int t0 = s.tok0; t0 < s.tok1; t0 += kTile) {
+      if (!dead && !ptx::mbar_wait(&full_bar[stage], phase, p.wait_ns)) {
+        if (lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+        dead = true;
+      }
+      if (t0 == s.tok0 && !dead) {
+        // Query rows as the B operand: lane (g, tig) holds head g, the dims of its K bytes.
+        const uint8_t* qs = base + L::q_off(NS) + stage * L::q_bytes(G);
+#pragma unroll
+        for (int hp = 0; hp < HP; ++hp)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int head = n * 8 + g;
+            if (head < G) {
+              const uint2* src = reinterpret_cast<const uint2*>(qs + ((size_t)(hp * G + head) * D + tig * (D / 4)) * 2);
+#pragma unroll
+              for (int i = 0; i < KS; ++i) {
+                const uint2 u = src[i];
+                qb[hp][n][i][0] = u.x;
+                qb[hp][n][i][1] = u.y;
+              }
+            }
+            if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+              // bf16 -> half, each head's row by a power of two that brings its largest value to
+              // 2^14..2^15: exact but for values under 2^-28 of that, undone after the product.
+              float mx = 0.f;
+#pragma unroll
+              for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  mx = fmaxf(mx, fabsf(__uint_as_float(qb[hp][n][i][k] << 16)));
+                  mx = fmaxf(mx, fabsf(__uint_as_float(qb[hp][n][i][k] & 0xffff0000u)));
+                }
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+              int e = (int)(__float_as_uint(mx) >> 23);
+              e = e < 15 ? 15 : e;
+              const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+              const float down = __uint_as_float((uint32_t)(e - 14) << 23) * p.scale_log2;
+#pragma unroll
+              for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const uint32_t u = qb[hp][n][i][k];
+                  qb[hp][n][i][k] =
+                      DT<__half>::pack2(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
+                }
+              hs[hp][n][0] = __shfl_sync(0xffffffffu, down, tig * 8);
+              hs[hp][n][1] = __shfl_sync(0xffffffffu, down, tig * 8 + 4);
+            }
+          }
+      }
+      const int left = s.tok1 - t0 - warp * 16;  // live tokens from this warp's first row on
+      if (left > 0 && !dead) {
+        const uint8_t* kp = base + stage * 2 * L::kPart + warp * 16 * ROWB;
+        const uint8_t* vp = kp + L::kPart;
+        const float* sc = reinterpret_cast<const float*>(base + L::scales_off(NS) + stage * kScaleFloats * 4);
+        const int j0 = warp * 16 / (kTile / nb);  // block of this warp's first row
+        const bool partial = left < 16;
+#pragma unroll
+        for (int hp = 0; hp < HP; ++hp) {
+          // ---- S^T = K Q^T
+          float st[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = st[n][2] = st[n][3] = 0.f;
+          uint32_t ka[D / 16], kb[D / 16];  // D / 4 bytes of rows g and g + 8
+          if constexpr (D >= 64) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              const uint32_t off = row_off<ROWB>(tk, hp * D + tig * (D / 4) + c * 16);
+              const uint4 a = *reinterpret_cast<const uint4*>(kp + off);
+              const uint4 b = *reinterpret_cast<const uint4*>(kp + off + 8 * ROWB);
+              ka[c * 4] = a.x, ka[c * 4 + 1] = a.y, ka[c * 4 + 2] = a.z, ka[c * 4 + 3] = a.w;
+              kb[c * 4] = b.x, kb[c * 4 + 1] = b.y, kb[c * 4 + 2] = b.z, kb[c * 4 + 3] = b.w;
+            }
+          } else {
+            const uint32_t off = row_off<ROWB>(tk, hp * D + tig * 8);
+            const uint2 a = *reinterpret_cast<const uint2*>(kp + off);
+            const uint2 b = *reinterpret_cast<const uint2*>(kp + off + 8 * ROWB);
+            ka[0] = a.x, ka[1] = a.y, kb[0] = b.x, kb[1] = b.y;
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const uint32_t a0 = q8::decode2(ka[i]), a2 = q8::decode2(ka[i] >> 16);
+            const uint32_t a1 = q8::decode2(kb[i]), a3 = q8::decode2(kb[i] >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) q8::mma16(st[n], a0, a1, a2, a3, qb[hp][n][i][0], qb[hp][n][i][1]);
+          }
+          // ---- scores, running maximum, weights
+          const float ks0 = sc[hp * nb + j0], ks1 = BS8 ? sc[hp * nb + j0 + 1] : ks0;
+          const float vs0 = sc[(HP + hp) * nb + j0], vs1 = BS8 ? sc[(HP + hp) * nb + j0 + 1] : vs0;
+          uint32_t pb[NT][2];
+          bool raise = false;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            st[n][0] *= ks0 * hs[hp][n][0];
+            st[n][1] *= ks0 * hs[hp][n][1];
+            st[n][2] *= ks1 * hs[hp][n][0];
+            st[n][3] *= ks1 * hs[hp][n][1];
+            if (partial) {
+              if (tk >= left) st[n][0] = st[n][1] = -INFINITY;
+              if (tk + 8 >= left) st[n][2] = st[n][3] = -INFINITY;
+            }
+            raise |= fmaxf(st[n][0], st[n][2]) > m[hp][n][0] + 8.f || fmaxf(st[n][1], st[n][3]) > m[hp][n][1] + 8.f;
+          }
+          // The maximum moves only when a score passes it by more than 2^8: weights stay
+          // below 2^8 (a half holds 2^16), and most tiles rescale nothing.
+          if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float mx = fmaxf(st[n][k], st[n][k + 2]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                mx = fmaxf(m[hp][n][k], mx);
+                const float c = mx == -INFINITY ? 1.f : ptx::ex2(m[hp][n][k] - mx);
+                m[hp][n][k] = mx;
+                l[hp][n][k] *= c;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                  o[hp][n][i][k] *= c;
+                  o[hp][n][i][k + 2] *= c;
+                }
+              }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float pr[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pr[k] = ptx::ex2(st[n][k] - m[hp][n][k & 1]);
+            l[hp][n][0] += pr[0] + pr[2];
+            l[hp][n][1] += pr[1] + pr[3];
+            pb[n][0] = q8::transpose8x8(DT<__half>::pack2(pr[0], pr[1]));
+            pb[n][1] = q8::transpose8x8(DT<__half>::pack2(pr[2], pr[3]));
+          }
+          // ---- O^T += v_scale (V^T P^T); lane (g, tig): D / 8 bytes of tokens tv0, tv1 and those + 8
+          constexpr int VW = D / 32;  // 32-bit words of a token
+          uint32_t v[4][VW];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int t = (k & 1 ? tv1 : tv0);
+            const uint8_t* src = vp + row_off<ROWB>(t, hp * D + g * (D / 8)) + (k >> 1) * 8 * ROWB;
+            if constexpr (VW == 4) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
+              v[k][0] = u.x, v[k][1] = u.y, v[k][2] = u.z, v[k][3] = u.w;
+            } else if constexpr (VW == 2) {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              v[k][0] = u.x, v[k][1] = u.y;
+            } else {
+              v[k][0] = *reinterpret_cast<const uint32_t*>(src);
+            }
+            if (partial && t + (k >> 1) * 8 >= left) {  // what lies behind the context may be NaN
+#pragma unroll
+              for (int x = 0; x < VW; ++x) v[k][x] = 0u;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < VW; ++x)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7362 : 0x5140;
+              const uint32_t lo = __byte_perm(v[0][x], v[1][x], sel), hi = __byte_perm(v[2][x], v[3][x], sel);
+              const uint32_t a0 = q8::decode2(lo), a1 = q8::decode2(lo >> 16);
+              const uint32_t a2 = q8::decode2(hi), a3 = q8::decode2(hi >> 16);
+              const int i = x * 2 + half;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (BS8) {
+                  float acc1[4] = {0.f, 0.f, 0.f, 0.f};
+                  q8::mma8(acc, a0, a1, pb[n][0]);
+                  q8::mma8(acc1, a2, a3, pb[n][1]);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) o[hp][n][i][k] = fmaf(vs1, acc1[k], o[hp][n][i][k]);
+                } else {
+                  q8::mma16(acc, a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[hp][n][i][k] = fmaf(vs0, acc[k], o[hp][n][i][k]);
+              }
+            }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&empty_bar[stage]);
+      if (++stage == NS) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---------------- the share's end: merge the four warps ----------------
+    ptx::named_barrier_sync(1, 128);  // all have read the previous merge
+#pragma unroll
+    for (int hp = 0; hp < HP; ++hp)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float sum = l[hp][n][k];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          const int head = n * 8 + tig * 2 + k;
+          if (head >= G) continue;
+          const int r = warp * R + hp * G + head;
+          if (g == 0) {
+            cm[r] = m[hp][n][k];
+            cl[r] = sum;
+          }
+          float2* dst = reinterpret_cast<float2*>(co + (size_t)r * D + g * (D / 8));
+#pragma unroll
+          for (int i = 0; i < KS; ++i) dst[i] = make_float2(o[hp][n][i][k], o[hp][n][i][k + 2]);
+        }
+    ptx::named_barrier_sync(1, 128);
+    T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * R) * D;
+    float* mine = s.n_parts == 1 ? nullptr : part_slot(p, blockIdx.x, (int)blockIdx.x == s.first_cta);
+    for (int i = threadIdx.x; i < R * D; i += 128) {
+      const int r = i / D;
+      float M = cm[r];
+#pragma unroll
+      for (int x = 1; x < 4; ++x) M = fmaxf(M, cm[x * R + r]);
+      float Lsum = 0.f, A = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        // a warp without tokens in this share has m = -inf and adds nothing
+        const float e = cm[x * R + r] == -INFINITY ? 0.f : ptx::ex2(cm[x * R + r] - M);
+        Lsum = fmaf(cl[x * R + r], e, Lsum);
+        A = fmaf(co[(size_t)x * R * D + i], e, A);
+      }
+      if (!mine) {
+        out[i] = DT<T>::from_f(A / Lsum);
+      } else {
+        __stcg(mine + i, A);
+        if (i % D == 0) {
+          __stcg(mine + R * D + r * 2, M);
+          __stcg(mine + R * D + r * 2 + 1, Lsum);
+        }
+      }
+    }
+    if (mine)
+      join_parts<T, D, 128>(p, s, s.b * heads + s.h, R, s.h * R, flag, threadIdx.x, [] { ptx::named_barrier_sync(1, 128); });
   }
 }
 
@@ -329,6 +771,73 @@ int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
   }
   TVK_CHECK_LAUNCH("paged_decode_q8_simt");
   return TVK_OK;
+}
+
+constexpr int kSmemPerCta = 112 * 1024;  // two CTAs on an SM
+
+template <typename T, int D, int HP, int NT, bool BS8>
+int launch_tc(Q8Params p, cudaStream_t stream) {
+  using L = TcLayout<D, HP>;
+  tvk::EncodeTiledFn encode = tvk::encode_tiled_fn();
+  if (!encode) {
+    tvk::set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return TVK_ERR_CUDA;
+  }
+  const cuuint64_t row = (cuuint64_t)p.n_kv_heads * D;
+  const cuuint64_t dims[3] = {row, (cuuint64_t)p.block_size, (cuuint64_t)p.num_blocks};
+  const cuuint64_t strides[2] = {row, row * p.block_size};
+  const cuuint32_t box[3] = {(cuuint32_t)L::ROWB, (cuuint32_t)(p.block_size < kTile ? p.block_size : kTile), 1u};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  const CUtensorMapSwizzle sw = L::ROWB == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : L::ROWB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUtensorMap tm[2];
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = encode(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(i ? p.v_cache : p.k_cache), dims,
+                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+      tvk::set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+      return TVK_ERR_CUDA;
+    }
+  }
+  // as many stages as fit twice on an SM, 8 at most
+  p.n_stages = 2;
+  while (p.n_stages < 8 && L::bytes(p.n_stages + 1, p.group) <= kSmemPerCta) ++p.n_stages;
+  const int smem = L::bytes(p.n_stages, p.group);
+  auto kern = paged_decode_q8_tc_kernel<T, D, HP, NT, BS8>;
+  int dev = 0;
+  TVK_CHECK_CUDA(cudaGetDevice(&dev));
+  static std::atomic<unsigned long long> attr_set{0};  // one bit per device
+  if (dev >= 64 || !(attr_set.load() >> dev & 1)) {
+    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerCta));
+    if (dev < 64) attr_set.fetch_or(1ull << dev);
+  }
+  const long long most =
+      (long long)p.batch * (p.n_kv_heads / HP) * ((p.max_ctx_tokens + kTile - 1) / kTile + kUnitTiles);
+  const long long pieces = (most + kMinPiece - 1) / kMinPiece;
+  const int grid = (int)(pieces < kTcCtas ? pieces : kTcCtas);
+  TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, kTcThreads, smem, stream, p, tm[0], tm[1]));
+  TVK_CHECK_LAUNCH("paged_decode_q8_tc");
+  return TVK_OK;
+}
+
+template <typename T, int D, int HP>
+int launch_heads(const Q8Params& p, cudaStream_t stream) {
+  const bool bs8 = p.block_size == 8;
+  if (p.group <= 8) return bs8 ? launch_tc<T, D, HP, 1, true>(p, stream) : launch_tc<T, D, HP, 1, false>(p, stream);
+  return bs8 ? launch_tc<T, D, HP, 2, true>(p, stream) : launch_tc<T, D, HP, 2, false>(p, stream);
+}
+
+// 16-bit queries on the tensor cores where 64-token tiles are whole blocks or lie in one.
+template <typename T>
+int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
+  const int bs = p.block_size;
+  if (!(bs == 8 || bs == 16 || bs == 32 || bs % kTile == 0)) return launch_simt<T>(p, head_dim, stream);
+  if (head_dim == 128) return launch_heads<T, 128, 1>(p, stream);
+  if (head_dim == 64)
+    return p.n_kv_heads % 2 == 0 ? launch_heads<T, 64, 2>(p, stream) : launch_heads<T, 64, 1>(p, stream);
+  return p.n_kv_heads % 4 == 0 ? launch_heads<T, 32, 4>(p, stream) : launch_heads<T, 32, 1>(p, stream);
 }
 
 }  // namespace
@@ -397,10 +906,13 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
   }
   p.max_ctx_tokens = blocks * block_size;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
+  const tvk::WaitTest wt = tvk::take_wait_test();
+  p.wait_ns = wt.armed ? wt.limit_ns : tvk::kDefaultWaitNs;
+  p.drop_loads = wt.armed ? 1 : 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case TVK_DTYPE_F16: return launch_simt<__half>(p, head_dim, s);
-    case TVK_DTYPE_BF16: return launch_simt<__nv_bfloat16>(p, head_dim, s);
+    case TVK_DTYPE_F16: return launch_16bit<__half>(p, head_dim, s);
+    case TVK_DTYPE_BF16: return launch_16bit<__nv_bfloat16>(p, head_dim, s);
     default: return launch_simt<float>(p, head_dim, s);
   }
 }
