@@ -75,14 +75,14 @@ def write_kv_slots(x, slots, codes, scale):
 
 
 def paged_decode(q, k_codes, v_codes, k_scale, v_scale, tables, ctx, max_context_len=None):
-    """q [B,1,Hq,D] -> (out, sum_t p_t |v_t|, max_t sum_d |q_d k_td| / sqrt(D), max |v|), the last three
-    for error bounds, per output element, head and head."""
+    """q [B,1,Hq,D] -> (out, sum_t p_t |v_t|, max_t sum_d |q_d k_td| / sqrt(D), max_d |q_d| max_t sum_d |k_td| / sqrt(D),
+    max |v|): the output, and for error bounds per output element, and per head."""
     q = np.asarray(q, dtype=np.float64)
     B, _, hq, d = q.shape
     n, bs, hkv = k_codes.shape[:3]
     g = hq // hkv
     out, mass = np.zeros_like(q), np.zeros_like(q)
-    span, vmax = np.zeros((B, hq)), np.zeros((B, hq))
+    span, wide, vmax = np.zeros((B, hq)), np.zeros((B, hq)), np.zeros((B, hq))
     width = tables.shape[1]
     if max_context_len is not None:
         width = min(width, -(-max_context_len // bs))
@@ -104,8 +104,9 @@ def paged_decode(q, k_codes, v_codes, k_scale, v_scale, tables, ctx, max_context
             out[b, 0, h] = p @ vh
             mass[b, 0, h] = p @ np.abs(vh)
             span[b, h] = (np.abs(kh) @ np.abs(q[b, 0, h])).max() / math.sqrt(d)
+            wide[b, h] = np.abs(q[b, 0, h]).max() * np.abs(kh).sum(-1).max() / math.sqrt(d)
             vmax[b, h] = np.abs(vh).max()
-    return out, mass, span, vmax
+    return out, mass, span, wide, vmax
 
 
 def token_logprobs(logits, tokens, top_k):

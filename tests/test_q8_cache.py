@@ -5,9 +5,12 @@ bounded per element by what the kernel rounds (u = half a step of the output typ
   u |out|                          the output's rounding
   2^-10 sum p|v|                   weights as halves before P.V (16-bit queries): 2^-11 on the weight, and
                                    the sum that normalises them is not rounded, so twice that at most
-  2 ds sum p|v|                    fp32 scores off by ds = (D + 16) 2^-23 max_t sum_d |q k| / sqrt(D)
+  2 ds sum p|v|                    fp32 scores off by ds = (D + 16) 2^-23 max_t sum_d |q k| / sqrt(D), and with 16-bit
+                                   queries by 2^-25 max|q| max_t sum_d |k| / sqrt(D): a query row, its maximum scaled to
+                                   2^7 or more, is a sum of e4m3 parts, the last scaled by 2^8, down to half of 2^-17
   (n + 16) 2^-23 sum p|v|          n fp32 additions in the output and in the normaliser
-  n 2^-24 max|v|                   weights below the smallest normal half
+  n 2^-23 max|v|                   weights below half the last step of their parts (2^-18, where the largest counts as
+                                   2^4 or more: 2^-23 of the largest)
 """
 
 import math
@@ -62,11 +65,13 @@ def _expect(c, mcl=None):
 
 
 def _bound(c, ref):
-    out, mass, span, vmax = ref
+    out, mass, span, wide, vmax = ref
     n = int(c["ctx"].max())
     ds = (c["d"] + 16) * 2.0 ** -23 * span[:, None, :, None]
+    if c["q"].dtype != torch.float32:
+        ds = ds + 2.0 ** -25 * wide[:, None, :, None]
     p = 2.0 ** -10 if c["q"].dtype != torch.float32 else 0.0
-    return U[c["q"].dtype] * np.abs(out) * (1 + 2.0 ** -6) + (p + 2 * ds + (n + 16) * 2.0 ** -23) * mass + n * 2.0 ** -24 * vmax[:, None, :, None]
+    return U[c["q"].dtype] * np.abs(out) * (1 + 2.0 ** -6) + (p + 2 * ds + (n + 16) * 2.0 ** -23) * mass + n * 2.0 ** -23 * vmax[:, None, :, None]
 
 
 def _check(c, got, mcl=None, ref=None):

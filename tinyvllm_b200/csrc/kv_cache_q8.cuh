@@ -25,16 +25,17 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Two e4m3 codes (16 bits) -> two halves; every code is a half exactly.
-__device__ __forceinline__ uint32_t decode2(uint32_t codes) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(codes));
-  return r;
+// Four e4m3 codes -> four halves (lo: codes 0 and 1); every code is a half exactly.
+__device__ __forceinline__ void decode4h(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 
 // Four codes -> four floats.
 __device__ __forceinline__ void decode4(uint32_t codes, float* f) {
-  const uint32_t lo = decode2(codes), hi = decode2(codes >> 16);
+  uint32_t lo, hi;
+  decode4h(codes, lo, hi);
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   f[0] = a.x;
@@ -60,24 +61,22 @@ __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
 }
 
-// 8x8 transpose of 16-bit elements across a warp.
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+// Two halves -> two e4m3 codes, nearest, ties to even.
+__device__ __forceinline__ uint32_t encode2h(uint32_t h) {
   uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f16x2 c, %1;\n\tcvt.u32.u16 %0, c;\n\t}" : "=r"(r) : "r"(h));
   return r;
 }
-
-// c += a * b, halves in, fp32 sums: 16 x 8 x 16 and 16 x 8 x 8.
-__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Two e4m3 codes (low 16 bits) -> two halves.
+__device__ __forceinline__ uint32_t decode2h(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
 }
-__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+__device__ __forceinline__ uint32_t sub2h(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 }  // namespace q8

@@ -4,13 +4,12 @@
 //   s_t = k_scale[blk(t), h] * (q . kcode_t) / sqrt(D)
 //   out = sum_t softmax(s)_t * v_scale[blk(t), h] * vcode_t,   t < min(context, table)
 //
-// The scales never touch the codes: a score is scaled after its dot product and
-// a block's share of the output after its P.V, both in fp32, so codes go to the
-// arithmetic exactly (every e4m3 value is a half) whatever the scales are.
+// The scales never touch the codes: a score is scaled after its dot product, and
+// a block's v_scale goes into the weights of its tokens, both in fp32.
 //
 // Work split.  The live tokens of all (sequence, KV head) units are laid out on
-// one line in tiles of 64 tokens (plus a few tiles' worth per unit for its start
-// and end) and cut into equal pieces, one per CTA; heads of a sequence lie next
+// one line in tiles of tokens (plus a few tiles' worth per unit for its start and
+// end) and cut into equal pieces, one per CTA; heads of a sequence lie next
 // to each other.  Every CTA works its piece out of the context lengths alone.  A
 // unit that lies in one piece is written at once; one cut by a border leaves fp32
 // partials (max, sum, unnormalised output) in the workspace, and the CTA that
@@ -22,16 +21,18 @@
 #include <type_traits>
 
 #include "kv_cache_q8.cuh"
+#include "sm100_umma.cuh"
 
 namespace {
 
-constexpr int kTile = 64;            // tokens per tile of the work line
-constexpr int kSimtTile = 32;        // tokens the simt kernel stages at a time
+constexpr int kSimtTile = 32;        // tokens the simt kernel stages at a time, and its tile of the work line
+constexpr int kTcTile = 128;         // the same for the tensor-core kernel: the rows of a matrix instruction
 constexpr int kMaxGroup = 16;        // query heads per KV head
-constexpr int kMaxCtas = 592;        // pieces a call is cut into at most (four CTAs on each of 148 SMs)
-constexpr int kTcCtas = 296;         // the same for the tensor-core kernel: two CTAs on each SM
+constexpr int kMaxCtas = 592;        // pieces a call is cut into at most (simt: four CTAs on each of 148 SMs)
+constexpr int kTcCtas = 296;         // tensor-core kernel: two CTAs on each SM
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
-constexpr int kMinPiece = 4;         // shortest piece, in tiles
+constexpr int kMinPiece = 2;         // shortest piece, in tiles
+constexpr int kMaxParts = 4;         // units per (sequence, KV head) at most, see group_splits
 constexpr int kSlotFloats = 2240;    // partials of one cut unit: rows * (D + 2), at most 64 * 34, 32 * 66 or 16 * 130
 
 struct Q8Params {
@@ -43,7 +44,7 @@ struct Q8Params {
   const float *k_scale, *v_scale;
   int* status;
   float* part;     // [2 * kMaxCtas][kSlotFloats]
-  int* counters;   // [batch * n_kv_heads], zero between calls
+  int* counters;   // [batch * n_kv_heads * kMaxParts], zero between calls
   int batch, n_heads, n_kv_heads, group, block_size, num_blocks, max_blocks;
   int max_ctx_tokens;
   float scale_log2;            // log2(e) / sqrt(head_dim)
@@ -56,7 +57,7 @@ __device__ __forceinline__ int effective_ctx(const Q8Params& p, int b) {
   const int c = p.context_lens[b];
   return c < 0 ? 0 : (c < p.max_ctx_tokens ? c : p.max_ctx_tokens);
 }
-__device__ __forceinline__ int tiles_of(int ctx) { return (ctx + kTile - 1) / kTile; }
+__host__ __device__ __forceinline__ int tiles_of(int ctx, int tile) { return (ctx + tile - 1) / tile; }
 
 // One CTA's share of one unit: tokens [tok0, tok1) of (b, h).  A unit without
 // context is one share with tok0 == tok1 and n_parts 1.
@@ -68,6 +69,7 @@ struct Share {
 
 // Walks the units of this CTA's piece.  `heads` = units per sequence.  All
 // members are the same in every lane of the calling warp.
+template <int TILE>
 struct Walker {
   long long x0, x1, total;
   int pieces, heads;
@@ -78,7 +80,7 @@ struct Walker {
   __device__ void start(const Q8Params& p, int heads_, int lane) {
     heads = heads_;
     long long sum = 0;
-    for (int i = lane; i < p.batch; i += 32) sum += tiles_of(effective_ctx(p, i)) + kUnitTiles;
+    for (int i = lane; i < p.batch; i += 32) sum += tiles_of(effective_ctx(p, i), TILE) + kUnitTiles;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     total = sum * heads;
@@ -92,7 +94,7 @@ struct Walker {
     for (int i0 = 0; i0 < p.batch; i0 += 32) {
       const int i = i0 + lane;
       const int c = i < p.batch ? effective_ctx(p, i) : 0;
-      const long long w = i < p.batch ? (long long)(tiles_of(c) + kUnitTiles) * heads : 0;
+      const long long w = i < p.batch ? (long long)(tiles_of(c, TILE) + kUnitTiles) * heads : 0;
       long long incl = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -109,7 +111,7 @@ struct Walker {
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    const int w = tiles_of(ctx) + kUnitTiles;
+    const int w = tiles_of(ctx, TILE) + kUnitTiles;
     h = (int)((x0 - at) / w);
     at += (long long)h * w;
   }
@@ -120,14 +122,14 @@ struct Walker {
   // The next share of the piece; false when there is none left.
   __device__ bool next(const Q8Params& p, Share& s) {
     while (b < p.batch && at < x1) {
-      const int tiles = tiles_of(ctx);
+      const int tiles = tiles_of(ctx, TILE);
       const long long lo = max(x0 - at, 0LL), hi = min(x1 - at, (long long)tiles);
       const bool mine = tiles ? lo < hi : lo == 0;
       s.b = b;
       s.h = h;
       s.ctx = ctx;
-      s.tok0 = (int)lo * kTile;
-      s.tok1 = min((int)hi * kTile, ctx);
+      s.tok0 = (int)lo * TILE;
+      s.tok1 = min((int)hi * TILE, ctx);
       s.first_cta = blockIdx.x;
       s.n_parts = 1;
       if (tiles && (lo > 0 || hi < tiles)) {
@@ -154,12 +156,11 @@ __device__ __forceinline__ float* part_slot(const Q8Params& p, int cta, bool is_
   return p.part + (size_t)(cta * 2 + (is_first ? 1 : 0)) * kSlotFloats;
 }
 
-// The end of a cut unit's share, by the NT threads that have just stored its
-// partials with __stcg (o [rows][D], then m, l [rows][2]): counts the arrival, and
-// the last to arrive adds the parts up and writes the output rows (query heads from
-// row0 on).  `flag` is a shared int; `sync` a barrier of the NT threads.
-template <typename T, int D, int NT, typename Sync>
-__device__ void join_parts(const Q8Params& p, const Share& s, int unit, int rows, int row0, int* flag, int tid, Sync sync) {
+// Counts the arrival of a share of a cut unit whose partials the calling threads
+// have just stored with __stcg; true in all of them for the last to arrive.
+// `flag` is a shared int; `sync` a barrier of these threads.
+template <typename Sync>
+__device__ bool last_to_arrive(const Q8Params& p, const Share& s, int unit, int* flag, int tid, Sync sync) {
   __threadfence();
   sync();
   if (tid == 0) {
@@ -169,22 +170,23 @@ __device__ void join_parts(const Q8Params& p, const Share& s, int unit, int rows
     __threadfence();
   }
   sync();
-  if (!*flag) return;
-  T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + row0) * D;
-  for (int i = tid; i < rows * D; i += NT) {
-    const int r = i / D;
-    float M = -INFINITY;
-    for (int c = 0; c < s.n_parts; ++c)
-      M = fmaxf(M, __ldcg(part_slot(p, s.first_cta + c, c == 0) + rows * D + r * 2));
-    float L = 0.f, A = 0.f;
-    for (int c = 0; c < s.n_parts; ++c) {
-      const float* src = part_slot(p, s.first_cta + c, c == 0);
-      const float w = exp2f(__ldcg(src + rows * D + r * 2) - M);
-      L = fmaf(__ldcg(src + rows * D + r * 2 + 1), w, L);
-      A = fmaf(__ldcg(src + i), w, A);
-    }
-    out[i] = DT<T>::from_f(A / L);
+  return *flag != 0;
+}
+
+// Element i (of row r) of a cut unit's output from all its partials, each
+// [n_o] unnormalised sums and then (max, sum) of every row.
+__device__ __forceinline__ float joined(const Q8Params& p, const Share& s, int n_o, int i, int r) {
+  float M = -INFINITY;
+  for (int c = 0; c < s.n_parts; ++c) M = fmaxf(M, __ldcg(part_slot(p, s.first_cta + c, c == 0) + n_o + r * 2));
+  float L = 0.f, A = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < s.n_parts; ++c) {
+    const float* src = part_slot(p, s.first_cta + c, c == 0);
+    const float w = exp2f(__ldcg(src + n_o + r * 2) - M);
+    L = fmaf(__ldcg(src + n_o + r * 2 + 1), w, L);
+    A = fmaf(__ldcg(src + i), w, A);
   }
+  return A / L;
 }
 
 // -----------------------------------------------------------------------------
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
   __shared__ int flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, bs = p.block_size, Hkv = p.n_kv_heads;
-  Walker w;
+  Walker<kSimtTile> w;
   w.start(p, Hkv, lane);
   Share s;
   while (w.next(p, s)) {
@@ -318,99 +320,220 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
       __stcg(mine + G * D + i * 2, mfin[i]);
       __stcg(mine + G * D + i * 2 + 1, lfin[i]);
     }
-    join_parts<T, D, 128>(p, s, s.b * Hkv + s.h, G, s.h * G, &flag, tid, [] { __syncthreads(); });
+    if (last_to_arrive(p, s, s.b * Hkv + s.h, &flag, tid, [] { __syncthreads(); }))
+      for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(joined(p, s, G * D, i, i / D));
   }
 }
 
 // -----------------------------------------------------------------------------
-// Tensor-core kernel: 16-bit queries; block sizes 8, 16, 32 and multiples of 64.
+// tcgen05 kernel: 16-bit queries; block sizes 8, 16, 32, 64 and multiples of 128.
 //
-// A unit is HP neighbouring KV heads of one sequence (HP * D bytes a token, 128
-// where the head count allows), so that one TMA row is a whole 128-byte line also
-// for small heads.  One producer warp streams 64-token tiles of codes (and their
-// scales, by 4-byte asynchronous copies, and at a share's start its query rows)
-// through a ring of stages; four consumer warps take 16 tokens of a tile each:
-//   S^T [16 tokens, 8 heads] = K . Q^T    A = codes as halves, straight from their rows
-//   P^T                       = 2^(S^T - m) as halves, transposed in registers
-//   O^T [D, 8 heads]         += v_scale * (V^T . P^T)
-// Tokens and dims, not heads, are the 16-row side of the products: at 4 to 8
-// query heads per KV head that halves the matrix instructions and the accumulators.
-// The order of the k index of a product is free, so a lane takes 16 neighbouring
-// bytes of its row as four k steps and nothing is shuffled; for V a byte
-// permute pairs the same dim of two tokens.
+// A unit is HP = 128 / D neighbouring KV heads of one sequence, so that a token's
+// codes are one 128-byte row whatever D is, and up to GP query heads of each
+// (larger groups take several units).  The codes are matrix operands as TMA
+// lands them, 128 tokens a tile:
+//   S^T [128 tokens, 4 GP] = K . Q^T         per KV head; K rows are K-major (128 B swizzle)
+//   O^T [128 dims, 4 GP HP] += V^T . P^T     V rows read M-major; all heads at once, a head's
+//                                            dims times other heads' columns are not read
+// and what has more bits than e4m3 comes in parts, each a column (slot) of its own:
+//  * a query row, scaled by a power of two to a maximum in [2^7, 2^8), is
+//    q1 + q2 + q3 + 2^-8 q4, each part the e4m3 of what is left: 4 significant bits
+//    a part, exact for fp16 and bf16 down to 2^-18 of 2^7, i.e. 2^-25 of the maximum;
+//  * a weight 2^(s + log2 v_scale - M), at most 2^8, is rounded to a half and is
+//    p1 + p2 + 2^-8 p3: exact down to 2^-18, where the largest counts as 2^4..2^8.
+// The matrix unit sums in fp32.  So nothing is converted per K/V element: the work of
+// the CUDA cores is per (token, query head).  (Decoding the codes to halves for
+// mma.sync took 470 instructions per 16 tokens and 265 us where this takes 218 us:
+// 256 sequences of 128-4096 tokens, 32/8 heads of 128.  mma.sync on e4m3 itself
+// is converted to halves by the compiler on this architecture and took longer still.)
+//
+// Roles: warp 0 streams K and V tiles (TMA) and their scales (4-byte asynchronous
+// copies); warp 1 issues the products; warp 2 splits the query rows of the next share;
+// warps 4-7, a thread per token, turn S^T into weights, keep the sums of weights, and
+// at a share's end, a thread per dim, read O^T and write the output.
+// K and V tiles go through one ring of 16 KB slots in the order the products take
+// them, K(0) K(1) V(0) K(2) V(1) ..., so that a K tile's slot is free again as soon as
+// its S^T is there and not only after the weights and P.V.
+// M and the reference R of the sums are per query head, the same in all threads.
+// They move only when a weight would pass 2^8 (or a sum's term 2^64); then O^T is rescaled.
 // -----------------------------------------------------------------------------
-template <int ROWB>
-__device__ __forceinline__ uint32_t row_off(int t, int byte) {  // as the TMA swizzle of ROWB-byte rows lays it
-  const int x = ROWB == 128 ? (t & 7) : ROWB == 64 ? ((t >> 1) & 3) : ((t >> 2) & 1);
-  return t * ROWB + ((((byte >> 4) ^ x) << 4) | (byte & 15));
-}
+constexpr int kTcThreads = 256;
+constexpr int kScaleRing = 8;  // tiles whose scales are kept: a K slot comes round only when S^T of 5 tiles later is read
+constexpr float kLowPart = 0.00390625f;
 
-constexpr int kTcThreads = 160;
-constexpr int kScaleFloats = 64;  // scales per stage: K and V, HP <= 4 heads, <= 8 blocks
-
-template <int D, int HP>
+template <int D, int GP>
 struct TcLayout {
-  static constexpr int ROWB = D * HP;
-  static constexpr int kPart = kTile * ROWB;  // K (or V) codes of a stage
-  // stage = K codes, V codes, scales, query rows
-  static __host__ __device__ int q_bytes(int group) { return HP * group * D * 2; }
-  static __host__ __device__ int scales_off(int n_stages) { return n_stages * 2 * kPart; }
-  static __host__ __device__ int q_off(int n_stages) { return scales_off(n_stages) + n_stages * kScaleFloats * 4; }
-  static __host__ __device__ int merge_off(int n_stages, int group) { return q_off(n_stages) + n_stages * q_bytes(group); }
-  // merge: o [4][HP * group][D], m, l and weights [4][HP * group], one flag
-  static __host__ __device__ int bar_off(int n_stages, int group) {
-    return merge_off(n_stages, group) + 4 * HP * group * (D + 3) * 4 + 16;
-  }
-  static __host__ __device__ int bytes(int n_stages, int group) { return bar_off(n_stages, group) + n_stages * 16 + 1024; }
+  static constexpr int HP = 128 / D;
+  static constexpr int HG = HP * GP;                    // query heads of a unit
+  static constexpr int NS = 4 * GP;                     // columns of S^T of one KV head: (part, head)
+  static constexpr int NO = (3 * HG + 15) / 16 * 16;    // columns of O^T: (part, KV head, head)
+  static constexpr int kOCol = 2 * HP * NS;             // after two buffers of S^T
+  static constexpr int kTmemCols = kOCol + NO <= 64 ? 64 : kOCol + NO <= 128 ? 128 : 256;
+  static constexpr int kSlot = kTcTile * 128;           // K or V codes of a tile
+  static constexpr int kQ = HP * NS * 128;              // query parts, one row of 128 B per column
+  static constexpr int kQBufs = HG == 16 ? 1 : 2;
+  static constexpr int kP = NO * 128;                   // weight parts: one row of 128 tokens per column
+  static constexpr int kScale = 2 * HP * 16 * 4;        // K and V, HP heads, <= 16 blocks
+  static constexpr int kMisc = 1536, kBars = 320;
+  static constexpr int kFixed = kQBufs * kQ + 2 * kP + kScaleRing * kScale + kMisc + kBars + 1024;
+  static constexpr int kSlots = (113 * 1024 - kFixed) / kSlot;  // two CTAs on an SM
+  static constexpr int kQOff = kSlots * kSlot;
+  static constexpr int kPOff = kQOff + kQBufs * kQ;
+  static constexpr int kScaleOff = kPOff + 2 * kP;
+  static constexpr int kMiscOff = kScaleOff + kScaleRing * kScale;
+  static constexpr int kBarOff = kMiscOff + kMisc;
+  static constexpr int kBytes = kBarOff + kBars + 1024;
+  static_assert(HG <= 16 && kOCol + NO <= 256 && kSlots >= 5 && kSlots <= 7, "sizes");
+  static_assert((2 * kSlots + kScaleRing + 14) * 8 <= kBars, "barriers");
+  static_assert(2 * kP / 4 >= HG * kTcCtas / 4, "room for the join's factors, a quarter of the parts at a time");
 };
 
-template <typename T, int D, int HP, int NT, bool BS8>
+// Byte of row r of a tile with 128-byte rows in the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swz128(int r, int byte) {
+  return r * 128 + ((((byte >> 4) ^ (r & 7)) & 7) << 4) + (byte & 15);
+}
+
+// Four neighbouring values -> q1, q2, q3 and 2^8 (what is left), e4m3, four bytes each.
+__device__ __forceinline__ void split_query(float (&x)[4], uint32_t (&w)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k == 3) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= 256.f;
+    }
+    w[k] = q8::encode2(x[0], x[1]) | (q8::encode2(x[2], x[3]) << 16);
+    float f[4];
+    q8::decode4(w[k], f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] -= f[i];
+  }
+}
+
+// Or of a flag over the 128 threads of warps 4-7.
+__device__ __forceinline__ bool any_of_128(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+// mbar_wait by a whole warp, one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, limit_ns));
+}
+
+// Largest value of a warp (NaN only where all are).
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename T, int D, int GP>
 __global__ void __launch_bounds__(kTcThreads, 2)
     paged_decode_q8_tc_kernel(const Q8Params p, const __grid_constant__ CUtensorMap tm_k,
                               const __grid_constant__ CUtensorMap tm_v) {
-  using L = TcLayout<D, HP>;
-  constexpr int ROWB = L::ROWB;
-  constexpr int KS = D / 16;  // k steps of S, and 16-dim tiles of O
+  using L = TcLayout<D, GP>;
+  constexpr int HP = L::HP, HG = L::HG, SL = L::kSlots, QB = L::kQBufs;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base_u32 = (raw + 1023u) & ~1023u;
   uint8_t* base = smem_raw + (base_u32 - raw);
-  const int G = p.group, NS = p.n_stages;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(base + ((L::bar_off(NS, G) + 7) & ~7));
-  uint64_t* empty_bar = full_bar + NS;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::kBarOff);
+  uint64_t* full_bar = bars;                 // [SL] slot's tile landed
+  uint64_t* empty_bar = full_bar + SL;       // [SL] slot's products done
+  uint64_t* sc_full = empty_bar + SL;        // [kScaleRing] a tile's scales landed
+  uint64_t* s_full = sc_full + kScaleRing;   // [2] S^T written
+  uint64_t* s_empty = s_full + 2;            // [2] S^T and the tile's scales read
+  uint64_t* p_full = s_empty + 2;            // [2] weights written
+  uint64_t* p_empty = p_full + 2;            // [2] P.V done
+  uint64_t* q_full = p_empty + 2;            // [QB] query parts written
+  uint64_t* q_empty = q_full + 2;            // [QB] the share's S^T all done, query factors read
+  uint64_t* o_empty = q_empty + 2;           // O^T read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
+  // misc: query factors [2][16], warp results [4][16][2], per head M, R, two factors [4][16], a flag
+  float* hs_s = reinterpret_cast<float*>(base + L::kMiscOff);
+  float* red_s = hs_s + 32;
+  float* M_s = red_s + 128;
+  float* R_s = M_s + 16;
+  float* c_s = R_s + 16;
+  float* lc_s = c_s + 16;
+  int* flag = reinterpret_cast<int*>(lc_s + 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) {
-      ptx::mbar_init(&full_bar[s], 33);  // the byte count, and every producer lane's scales
-      ptx::mbar_init(&empty_bar[s], 4);
+    for (int i = 0; i < SL; ++i) {
+      ptx::mbar_init(&full_bar[i], 1);
+      ptx::mbar_init(&empty_bar[i], 1);
     }
+    for (int i = 0; i < kScaleRing; ++i) ptx::mbar_init(&sc_full[i], 32);
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&s_empty[i], 4);
+      ptx::mbar_init(&p_full[i], 4);
+      ptx::mbar_init(&p_empty[i], 1);
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&q_empty[i], 5);
+    }
+    ptx::mbar_init(o_empty, 4);
     ptx::fence_mbar_init();
   }
+  if (warp == 1) {
+    umma::tmem_alloc(tmem_slot, L::kTmemCols);
+    umma::tmem_relinquish();
+  }
+  umma::fence_before_sync();
   __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int heads = p.n_kv_heads / HP;
-  Walker w;
-  w.start(p, heads, lane);
-  Share s;
-  int stage = 0;
-  uint32_t phase = 0;
 
-  if (warp == 4) {
+  const int G = p.group, Hkv = p.n_kv_heads;
+  const int pairs = (Hkv + HP - 1) / HP, splits = (G + GP - 1) / GP;
+  const int units = pairs * splits;
+  const int rows = p.block_size < kTcTile ? p.block_size : kTcTile;  // rows of one TMA box
+  const int nb = kTcTile / rows;                                     // blocks of a tile
+  Share s;
+  Walker<kTcTile> w;
+  if (warp != 3) w.start(p, units, lane);
+  // Slot of the n-th tile of the ring's order and the parity of its round.
+  auto slot_of = [](uint32_t n) { return n % SL; };
+  auto round_of = [](uint32_t n) { return (n / SL) & 1; };
+  // Places of K and V of tile number t in that order.
+  auto k_at = [](uint32_t t) { return t == 0 ? 0u : 2 * t - 1; };
+  // V(t) follows K(t + 1) if there is one: the last tile's V closes the order.
+  auto v_at = [](uint32_t t) { return 2 * t + 2; };
+
+  if (warp == 0) {
     // ---------------- producer ----------------
     if (lane == 0) {
       ptx::prefetch_tmap(&tm_k);
       ptx::prefetch_tmap(&tm_v);
     }
-    const int rows = p.block_size < kTile ? p.block_size : kTile;  // rows of one TMA box
-    const int nb = kTile / rows;                                   // blocks of a tile
-    const int q_bytes = L::q_bytes(G);
-    bool running = true;
-    while (running && w.next(p, s)) {
+    uint32_t it = 0;
+    bool ok = true;
+    // One code tile into the ring: lane j holds the id of the tile's block j.
+    auto load = [&](uint32_t n, const CUtensorMap* tm, int live, int x, int row, int blk) {
+      const uint32_t sl = slot_of(n);
+      ok = ok && warp_wait(&empty_bar[sl], round_of(n) ^ 1, p.wait_ns);
+      if (!ok || p.drop_loads) return;
+      if (lane == 0) ptx::mbar_arrive_expect_tx(&full_bar[sl], (uint32_t)(live * rows * 128));
+      __syncwarp();
+      if (lane < live)
+        q8::tma_load_3d(base_u32 + sl * L::kSlot + lane * rows * 128, tm, &full_bar[sl], x, row, blk);
+    };
+    int v_live = 0, v_x = 0, v_row = 0, v_blk = 0;
+    while (ok && w.next(p, s)) {
+      const int pair = s.h / splits;
       const int32_t* bt = p.block_tables + (size_t)s.b * p.max_blocks;
       const int blk_end = (s.tok1 + p.block_size - 1) / p.block_size;
       constexpr int W = 4;  // ids of 128 blocks at a time, one per lane and register
       int win = -W * 32, id[W];
-      for (int t0 = s.tok0; t0 < s.tok1; t0 += kTile) {
+      for (int t0 = s.tok0; ok && t0 < s.tok1; t0 += kTcTile) {
         const int first = t0 / p.block_size;
         if (first + nb > win + W * 32) {
           win = first;
@@ -420,348 +543,424 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             id[r] = i < blk_end ? __ldg(bt + i) : -1;
           }
         }
-        if (!ptx::mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_ns)) {
-          if (lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
-          running = false;
-          break;
+        const int live = min(nb, blk_end - first);
+        const int rel = first + lane % nb - win;
+        int blk = -1;
+#pragma unroll
+        for (int r = 0; r < W; ++r) {
+          const int v = __shfl_sync(0xffffffffu, id[r], rel & 31);
+          blk = (rel >> 5) == r ? v : blk;
         }
-        if (!p.drop_loads) {
-          const int live = min(nb, blk_end - first);
-          if (lane == 0) {
-            uint32_t tx = (uint32_t)(live * rows * ROWB * 2);
-            if (t0 == s.tok0) tx += q_bytes;
-            ptx::mbar_arrive_expect_tx(&full_bar[stage], tx);
-            if (t0 == s.tok0)
-              ptx::bulk_load(base + L::q_off(NS) + stage * q_bytes,
-                             reinterpret_cast<const uint8_t*>(p.q) + ((size_t)s.b * p.n_heads + (size_t)s.h * HP * G) * D * 2,
-                             (uint32_t)q_bytes, &full_bar[stage]);
+        load(k_at(it), &tm_k, live, pair * 128, t0 % p.block_size, blk);
+        if (ok && !p.drop_loads) {
+          // scales [K, V][HP][nb]: this lane's block, K / V and heads by turns
+          const uint32_t scales = base_u32 + L::kScaleOff + (it % kScaleRing) * L::kScale;
+          const int j = lane % nb;
+          for (int i = lane / nb; i < 2 * HP; i += 32 / nb) {
+            const int kv = i & 1, hp = i >> 1, head = pair * HP + hp;
+            const bool in = j < live && blk >= 0 && blk < p.num_blocks && head < Hkv;
+            const float* src = kv ? p.v_scale : p.k_scale;
+            q8::copy4_async(scales + ((kv * HP + hp) * nb + j) * 4, in ? src + (size_t)blk * Hkv + head : src, in);
           }
-          __syncwarp();
-          // lane = block of the tile (up to 8) and, for the scales, head and K / V
-          const uint32_t codes = base_u32 + stage * 2 * L::kPart;
-          const uint32_t scales = base_u32 + L::scales_off(NS) + stage * kScaleFloats * 4;
-          for (int i0 = 0; i0 < nb * 2 * HP; i0 += 32) {
-            const int i = i0 + lane, j = i % nb, kv = (i / nb) & 1, hp = i / (2 * nb);
-            const int rel = first + j - win;
-            int blk = -1;
-#pragma unroll
-            for (int r = 0; r < W; ++r) {
-              const int v = __shfl_sync(0xffffffffu, id[r], rel & 31);
-              blk = (rel >> 5) == r ? v : blk;
-            }
-            if (i < nb * 2 * HP) {
-              const bool in = j < live && blk >= 0 && blk < p.num_blocks;
-              const float* src = kv ? p.v_scale : p.k_scale;
-              q8::copy4_async(scales + ((kv * HP + hp) * nb + j) * 4,
-                              in ? src + (size_t)blk * p.n_kv_heads + s.h * HP + hp : src, in);
-              if (hp == 0 && j < live)
-                q8::tma_load_3d(codes + kv * L::kPart + j * rows * ROWB, kv ? &tm_v : &tm_k, &full_bar[stage],
-                                s.h * HP * D, t0 % p.block_size, blk);
-            }
-          }
-          q8::arrive_after_copies(&full_bar[stage]);
+          q8::arrive_after_copies(&sc_full[it % kScaleRing]);
         }
-        if (++stage == NS) {
-          stage = 0;
-          phase ^= 1;
-        }
+        if (it > 0) load(v_at(it - 1), &tm_v, v_live, v_x, v_row, v_blk);
+        v_live = live;
+        v_x = pair * 128;
+        v_row = t0 % p.block_size;
+        v_blk = blk;
+        ++it;
       }
     }
-    // No copy is in flight when the CTA ends, whatever became of the consumers.
-    for (int i = 0; i < NS && !p.drop_loads; ++i) {
-      if (!ptx::mbar_wait(&full_bar[stage], phase ^ 1, p.wait_ns)) break;
-      if (++stage == NS) {
-        stage = 0;
-        phase ^= 1;
+    uint32_t total = 0;
+    if (it > 0) {
+      total = v_at(it - 1);  // no K after the last tile: its place stays empty
+      load(total - 1, &tm_v, v_live, v_x, v_row, v_blk);
+    }
+    if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+    // No copy is in flight when the CTA ends, whatever became of the others.
+    for (uint32_t n = total > SL ? total - SL : 0; n < total && ok && !p.drop_loads; ++n)
+      ok = warp_wait(&full_bar[slot_of(n)], round_of(n), p.wait_ns);
+  } else if (warp == 1) {
+    // ---------------- matrix issue: S^T of a tile, then P.V of the one before ----------------
+    constexpr uint32_t idesc_s = umma::idesc_e4m3(128, L::NS, false);
+    constexpr uint32_t idesc_o = umma::idesc_e4m3(128, L::NO, true);
+    uint32_t it = 0, share = 0;
+    bool prev_first = false, ok = true;
+    // P.V of tile t, its V at place n, share sh
+    auto issue_pv = [&](uint32_t t, uint32_t n, bool first_of_share, uint32_t sh) {
+      const uint32_t b = t & 1, sl = slot_of(n);
+      ok = ok && warp_wait(&full_bar[sl], round_of(n), p.wait_ns);
+      if (first_of_share) ok = ok && warp_wait(o_empty, (sh & 1) ^ 1, p.wait_ns);
+      ok = ok && warp_wait(&p_full[b], (t >> 1) & 1, p.wait_ns);
+      if (!ok) return;
+      umma::fence_after_sync();
+      if (lane == 0) {
+        const uint32_t va = base_u32 + sl * L::kSlot, pa = base_u32 + L::kPOff + b * L::kP;
+#pragma unroll
+        for (int k = 0; k < kTcTile / 32; ++k)
+          umma::mma_f8_ss(tmem + L::kOCol, umma::smem_desc_sw128(va + k * 32 * 128, 0, 1024),
+                          umma::smem_desc_sw128(pa + k * 32, 0, 1024), idesc_o, !(first_of_share && k == 0));
+        umma::commit(&empty_bar[sl]);
+        umma::commit(&p_empty[b]);
       }
-    }
-    return;
-  }
-
-  // ---------------- consumers ----------------
-  const int g = lane >> 2, tig = lane & 3;
-  const int nb = p.block_size < kTile ? kTile / p.block_size : 1;
-  const int R = HP * G;  // output rows of a unit
-  float* co = reinterpret_cast<float*>(base + L::merge_off(NS, G));
-  float* cm = co + 4 * R * D;
-  float* cl = cm + 4 * R;
-  float* cw = cl + 4 * R;
-  int* flag = reinterpret_cast<int*>(cw + 4 * R);
-  // Row r of an 8-token group is token tok_of(r): an order in which the lanes of one
-  // shared-memory access fall on different banks.
-  auto tok_of = [](int r) { return HP == 1 ? r : HP == 2 ? (r >> 1) | ((r & 1) << 2) : ((r & 3) << 1) | (r >> 2); };
-  const int tk = tok_of(g), tv0 = tok_of(2 * tig), tv1 = tok_of(2 * tig + 1);
-  bool dead = false;  // a wait ran out: go through the motions, so that every counter is met
-
-  while (w.next(p, s)) {
-    if (s.ctx == 0) {
-      T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * R) * D;
-      for (int i = threadIdx.x; i < R * D; i += 128) out[i] = DT<T>::from_f(0.f);
-      continue;
-    }
-    uint32_t qb[HP][NT][KS][2];
-    float o[HP][NT][KS][4], m[HP][NT][2], l[HP][NT][2], hs[HP][NT][2];
+      __syncwarp();
+    };
+    while (ok && w.next(p, s)) {
+      if (s.tok0 == s.tok1) continue;
+      const uint32_t qb = share % QB;
+      for (int t0 = s.tok0; ok && t0 < s.tok1; t0 += kTcTile) {
+        const uint32_t b = it & 1, n = k_at(it), sl = slot_of(n);
+        if (t0 == s.tok0) ok = ok && warp_wait(&q_full[qb], (share / QB) & 1, p.wait_ns);
+        ok = ok && warp_wait(&s_empty[b], ((it >> 1) & 1) ^ 1, p.wait_ns);
+        ok = ok && warp_wait(&full_bar[sl], round_of(n), p.wait_ns);
+        if (!ok) break;
+        umma::fence_after_sync();
+        if (lane == 0) {
+          const uint32_t ka = base_u32 + sl * L::kSlot, qa = base_u32 + L::kQOff + qb * L::kQ;
 #pragma unroll
-    for (int hp = 0; hp < HP; ++hp)
+          for (int hp = 0; hp < HP; ++hp)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          o[hp][n][i][0] = o[hp][n][i][1] = o[hp][n][i][2] = o[hp][n][i][3] = 0.f;
-          qb[hp][n][i][0] = qb[hp][n][i][1] = 0u;
+            for (int k = 0; k < D / 32; ++k)
+              umma::mma_f8_ss(tmem + (b * HP + hp) * L::NS, umma::smem_desc_sw128(ka + hp * D + k * 32, 0, 1024),
+                              umma::smem_desc_sw128(qa + hp * L::NS * 128 + k * 32, 0, 1024), idesc_s, k > 0);
+          umma::commit(&s_full[b]);
+          umma::commit(&empty_bar[sl]);
+          if (t0 + kTcTile >= s.tok1) umma::commit(&q_empty[qb]);
         }
-        m[hp][n][0] = m[hp][n][1] = -INFINITY;
-        l[hp][n][0] = l[hp][n][1] = 0.f;
-        hs[hp][n][0] = hs[hp][n][1] = p.scale_log2;
+        __syncwarp();
+        if (it > 0) issue_pv(it - 1, v_at(it - 1), prev_first, t0 == s.tok0 ? share - 1 : share);
+        prev_first = t0 == s.tok0;
+        ++it;
       }
-    for (int t0 = s.tok0; t0 < s.tok1; t0 += kTile) {
-      if (!dead && !ptx::mbar_wait(&full_bar[stage], phase, p.wait_ns)) {
+      ++share;
+    }
+    if (ok && it > 0) {
+      issue_pv(it - 1, v_at(it - 1) - 1, prev_first, share - 1);
+      ok = ok && warp_wait(&p_empty[(it - 1) & 1], ((it - 1) >> 1) & 1, p.wait_ns);  // nothing runs when TMEM is freed
+    }
+    if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+  } else if (warp == 2) {
+    // ---------------- query rows of each share, in parts ----------------
+    constexpr int LPR = D / 4;     // lanes per row, four elements each
+    constexpr int RPW = 32 / LPR;  // rows at a time
+    uint32_t share = 0;
+    bool ok = true;
+    while (ok && w.next(p, s)) {
+      if (s.tok0 == s.tok1) continue;
+      const uint32_t qb = share % QB;
+      const int pair = s.h / splits, g0 = (s.h % splits) * GP;
+      // row i = (KV head, query head) of the unit
+      uint2 u[HG / RPW];
+#pragma unroll
+      for (int i = 0; i < HG / RPW; ++i) {
+        const int r = i * RPW + lane / LPR, hp = r / GP, h = g0 + r % GP, head = pair * HP + hp;
+        u[i] = make_uint2(0u, 0u);
+        if (h < G && head < Hkv)
+          u[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(p.q) +
+                                                 ((size_t)s.b * p.n_heads + (size_t)head * G + h) * D + (lane % LPR) * 4);
+      }
+      ok = warp_wait(&q_empty[qb], ((share / QB) & 1) ^ 1, p.wait_ns);
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < HG / RPW; ++i) {
+        const int r = i * RPW + lane / LPR, hp = r / GP, h = r % GP;
+        const T* e4 = reinterpret_cast<const T*>(&u[i]);
+        float x[4], mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = DT<T>::to_f(e4[k]);
+          mx = fmaxf(mx, fabsf(x[k]));
+        }
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        int e = (int)(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= mx
+        e = e < 8 ? 8 : e;
+        // to [2^7, 2^8); a row with an infinity is NaN altogether, as its softmax is
+        const float up = e == 255 ? __int_as_float(0x7fffffff) : __uint_as_float((uint32_t)(261 - e) << 23);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] *= up;
+        uint32_t parts[4];
+        split_query(x, parts);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint32_t*>(base + L::kQOff + qb * L::kQ + hp * L::NS * 128 +
+                                       swz128(k * GP + h, (lane % LPR) * 4)) = parts[k];
+        if (lane % LPR == 0) hs_s[qb * 16 + r] = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
+      }
+      umma::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&q_full[qb]);
+      ++share;
+    }
+    if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+  } else if (warp >= 4) {
+    // ---------------- weights (thread = token), output (thread = dim) ----------------
+    const int wq = warp - 4, tid = threadIdx.x - 128;
+    const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
+    const int my_block = tid / rows;            // block of this thread's token
+    const int my_hp = tid / D, dim = tid % D;   // KV head and dim of this thread's row of O^T
+    uint32_t it = 0, share = 0;
+    bool dead = false;  // a wait ran out: go through the motions, so that every counter is met
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!dead && !warp_wait(bar, parity, p.wait_ns)) {
         if (lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
         dead = true;
       }
-      if (t0 == s.tok0 && !dead) {
-        // Query rows as the B operand: lane (g, tig) holds head g, the dims of its K bytes.
-        const uint8_t* qs = base + L::q_off(NS) + stage * L::q_bytes(G);
+    };
+    // The next share with tokens; the rows of those without are zeros.
+    auto next_share = [&]() -> bool {
+      while (w.next(p, s)) {
+        if (s.ctx > 0) return true;
+        const int head = s.h / splits * HP + my_hp, g0 = (s.h % splits) * GP;
+        T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + (size_t)head * G + g0) * D + dim;
+        for (int h = 0; head < Hkv && h < min(GP, G - g0); ++h) out[(size_t)h * D] = DT<T>::from_f(0.f);
+      }
+      return false;
+    };
+    bool more = next_share();
+    while (more) {
+      const Share cur = s;
+      more = next_share();  // before this one is worked on, to know this CTA's last tile
+      const int pair = cur.h / splits, g0 = (cur.h % splits) * GP;
+      const int nh = min(GP, G - g0);  // query heads per KV head in this unit
+      T* out = reinterpret_cast<T*>(p.out) + (size_t)cur.b * p.n_heads * D;
+      const int head0 = (pair * HP + my_hp) * G + g0;  // this thread's first output head
+      const bool mine = pair * HP + my_hp < Hkv;
+      const uint32_t qb = share % QB;
+      if (tid < 16) M_s[tid] = R_s[tid] = -INFINITY;
+      wait(&q_full[qb], (share / QB) & 1);
+      float hs[HG], l[HG];
+#pragma unroll
+      for (int i = 0; i < HG; ++i) {
+        hs[i] = hs_s[qb * 16 + i];
+        l[i] = 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&q_empty[qb]);
+      ptx::named_barrier_sync(1, 128);  // M_s and R_s are set
+
+      for (int t0 = cur.tok0; t0 < cur.tok1; t0 += kTcTile) {
+        const uint32_t b = it & 1;
+        const bool live = t0 + tid < cur.tok1;
+        wait(&sc_full[it % kScaleRing], (it / kScaleRing) & 1);
+        const float* sc = reinterpret_cast<const float*>(base + L::kScaleOff + (it % kScaleRing) * L::kScale);
+        float ks[HP], lv[HP];  // k_scale and log2 v_scale of this thread's token
+#pragma unroll
+        for (int hp = 0; hp < HP; ++hp) {
+          ks[hp] = sc[hp * nb + my_block];
+          lv[hp] = live ? __log2f(sc[(HP + hp) * nb + my_block]) : 0.f;
+        }
+        wait(&s_full[b], (it >> 1) & 1);
+        umma::fence_after_sync();
+        float x[HG];  // scores, base 2
+        bool raise = false;
+#pragma unroll
+        for (int hp = 0; hp < HP; ++hp) {
+          float c0[GP], c1[GP], c2[GP], c3[GP];
+          const uint32_t at = lane_addr + (b * HP + hp) * L::NS;
+          umma::ld_32x32b<GP>(at, c0);
+          umma::ld_32x32b<GP>(at + GP, c1);
+          umma::ld_32x32b<GP>(at + 2 * GP, c2);
+          umma::ld_32x32b<GP>(at + 3 * GP, c3);
+          umma::ld_wait();
+#pragma unroll
+          for (int h = 0; h < GP; ++h) {
+            const int i = hp * GP + h;
+            const float sum = fmaf(c3[h], kLowPart, c2[h] + c1[h]) + c0[h];
+            x[i] = live ? sum * (ks[hp] * hs[i]) : -INFINITY;
+            if (h < nh) raise |= x[i] + lv[hp] > M_s[i] + 8.f || x[i] > R_s[i] + 64.f;
+          }
+        }
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s_empty[b]);
+        if (any_of_128(raise)) {
+          // New references: the largest weight so far counts as 2^4, the largest term of a sum as 1.
+#pragma unroll
+          for (int i = 0; i < HG; ++i) {
+            const float a = warp_max(x[i] + lv[i / GP]), c = warp_max(x[i]);
+            if (lane == 0) *reinterpret_cast<float2*>(red_s + (wq * 16 + i) * 2) = make_float2(a, c);
+          }
+          ptx::named_barrier_sync(1, 128);
+          if (tid < HG) {
+            float nm = M_s[tid], nr = R_s[tid];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              nm = fmaxf(nm, red_s[(k * 16 + tid) * 2] - 4.f);
+              nr = fmaxf(nr, red_s[(k * 16 + tid) * 2 + 1]);
+            }
+            c_s[tid] = nm == -INFINITY ? 1.f : ptx::ex2(M_s[tid] - nm);
+            lc_s[tid] = nr == -INFINITY ? 1.f : ptx::ex2(R_s[tid] - nr);
+            M_s[tid] = nm;
+            R_s[tid] = nr;
+          }
+          if (t0 != cur.tok0) wait(&p_empty[b ^ 1], ((it - 1) >> 1) & 1);  // P.V of the tile before: O^T is at rest
+          ptx::named_barrier_sync(1, 128);
+          umma::fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < HG; ++i) l[i] *= lc_s[i];
+          if (t0 != cur.tok0) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              float o[GP];
+              const uint32_t at = lane_addr + L::kOCol + k * HG + my_hp * GP;
+              umma::ld_32x32b<GP>(at, o);
+              umma::ld_wait();
+#pragma unroll
+              for (int h = 0; h < GP; ++h) o[h] *= c_s[my_hp * GP + h];
+              umma::st_32x32b<GP>(at, o);
+            }
+            umma::st_wait();
+            umma::fence_before_sync();
+          }
+        }
+        // Weights, their sums, and their parts as rows of P^T: this thread's token is byte tid.
+        wait(&p_empty[b], ((it >> 1) & 1) ^ 1);
+        uint8_t* pw = base + L::kPOff + b * L::kP;
 #pragma unroll
         for (int hp = 0; hp < HP; ++hp)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int head = n * 8 + g;
-            if (head < G) {
-              const uint2* src = reinterpret_cast<const uint2*>(qs + ((size_t)(hp * G + head) * D + tig * (D / 4)) * 2);
+          for (int h = 0; h < GP; h += 2) {
+            if (h >= nh) continue;
+            float wt[2];
 #pragma unroll
-              for (int i = 0; i < KS; ++i) {
-                const uint2 u = src[i];
-                qb[hp][n][i][0] = u.x;
-                qb[hp][n][i][1] = u.y;
-              }
+            for (int k = 0; k < 2; ++k) {
+              const int i = hp * GP + h + k;
+              const float M = M_s[i];
+              l[i] += ptx::ex2(x[i] - R_s[i]);
+              wt[k] = ptx::ex2(x[i] + lv[hp] - (M == -INFINITY ? 0.f : M));
             }
-            if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-              // bf16 -> half, each head's row by a power of two that brings its largest value to
-              // 2^14..2^15: exact but for values under 2^-28 of that, undone after the product.
-              float mx = 0.f;
+            const uint32_t hw = DT<__half>::pack2(wt[0], wt[1]);
+            const uint32_t c1 = q8::encode2h(hw), r1 = q8::sub2h(hw, q8::decode2h(c1));
+            const uint32_t c2 = q8::encode2h(r1), r2 = q8::sub2h(r1, q8::decode2h(c2));
+            const __half2 r3 = __hmul2(*reinterpret_cast<const __half2*>(&r2), __float2half2_rn(256.f));
+            const uint32_t c3 = q8::encode2h(*reinterpret_cast<const uint32_t*>(&r3));
+            const uint32_t cs[3] = {c1, c2, c3};
 #pragma unroll
-              for (int i = 0; i < KS; ++i)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  mx = fmaxf(mx, fabsf(__uint_as_float(qb[hp][n][i][k] << 16)));
-                  mx = fmaxf(mx, fabsf(__uint_as_float(qb[hp][n][i][k] & 0xffff0000u)));
-                }
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-              int e = (int)(__float_as_uint(mx) >> 23);
-              e = e < 15 ? 15 : e;
-              const float up = __uint_as_float((uint32_t)(268 - e) << 23);
-              const float down = __uint_as_float((uint32_t)(e - 14) << 23) * p.scale_log2;
-#pragma unroll
-              for (int i = 0; i < KS; ++i)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const uint32_t u = qb[hp][n][i][k];
-                  qb[hp][n][i][k] =
-                      DT<__half>::pack2(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
-                }
-              hs[hp][n][0] = __shfl_sync(0xffffffffu, down, tig * 8);
-              hs[hp][n][1] = __shfl_sync(0xffffffffu, down, tig * 8 + 4);
+            for (int k = 0; k < 3; ++k) {
+              const int row = k * HG + hp * GP + h;
+              pw[swz128(row, tid)] = (uint8_t)cs[k];
+              if (h + 1 < nh) pw[swz128(row + 1, tid)] = (uint8_t)(cs[k] >> 8);
             }
           }
-      }
-      const int left = s.tok1 - t0 - warp * 16;  // live tokens from this warp's first row on
-      if (left > 0 && !dead) {
-        const uint8_t* kp = base + stage * 2 * L::kPart + warp * 16 * ROWB;
-        const uint8_t* vp = kp + L::kPart;
-        const float* sc = reinterpret_cast<const float*>(base + L::scales_off(NS) + stage * kScaleFloats * 4);
-        const int j0 = warp * 16 / (kTile / nb);  // block of this warp's first row
-        const bool partial = left < 16;
+        // What lies behind the context has no weight, but may be NaN: zeros for V.
+        if (t0 + kTcTile > cur.tok1) {
+          const bool last = !more && t0 + kTcTile >= cur.tok1;
+          const uint32_t n = v_at(it) - (last ? 1 : 0);
+          wait(&full_bar[slot_of(n)], round_of(n));
+          if (!live) {
+            uint4* v = reinterpret_cast<uint4*>(base + slot_of(n) * L::kSlot + tid * 128);
 #pragma unroll
-        for (int hp = 0; hp < HP; ++hp) {
-          // ---- S^T = K Q^T
-          float st[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = st[n][2] = st[n][3] = 0.f;
-          uint32_t ka[D / 16], kb[D / 16];  // D / 4 bytes of rows g and g + 8
-          if constexpr (D >= 64) {
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              const uint32_t off = row_off<ROWB>(tk, hp * D + tig * (D / 4) + c * 16);
-              const uint4 a = *reinterpret_cast<const uint4*>(kp + off);
-              const uint4 b = *reinterpret_cast<const uint4*>(kp + off + 8 * ROWB);
-              ka[c * 4] = a.x, ka[c * 4 + 1] = a.y, ka[c * 4 + 2] = a.z, ka[c * 4 + 3] = a.w;
-              kb[c * 4] = b.x, kb[c * 4 + 1] = b.y, kb[c * 4 + 2] = b.z, kb[c * 4 + 3] = b.w;
-            }
-          } else {
-            const uint32_t off = row_off<ROWB>(tk, hp * D + tig * 8);
-            const uint2 a = *reinterpret_cast<const uint2*>(kp + off);
-            const uint2 b = *reinterpret_cast<const uint2*>(kp + off + 8 * ROWB);
-            ka[0] = a.x, ka[1] = a.y, kb[0] = b.x, kb[1] = b.y;
+            for (int k = 0; k < 8; ++k) v[k] = make_uint4(0u, 0u, 0u, 0u);
           }
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const uint32_t a0 = q8::decode2(ka[i]), a2 = q8::decode2(ka[i] >> 16);
-            const uint32_t a1 = q8::decode2(kb[i]), a3 = q8::decode2(kb[i] >> 16);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) q8::mma16(st[n], a0, a1, a2, a3, qb[hp][n][i][0], qb[hp][n][i][1]);
-          }
-          // ---- scores, running maximum, weights
-          const float ks0 = sc[hp * nb + j0], ks1 = BS8 ? sc[hp * nb + j0 + 1] : ks0;
-          const float vs0 = sc[(HP + hp) * nb + j0], vs1 = BS8 ? sc[(HP + hp) * nb + j0 + 1] : vs0;
-          uint32_t pb[NT][2];
-          bool raise = false;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            st[n][0] *= ks0 * hs[hp][n][0];
-            st[n][1] *= ks0 * hs[hp][n][1];
-            st[n][2] *= ks1 * hs[hp][n][0];
-            st[n][3] *= ks1 * hs[hp][n][1];
-            if (partial) {
-              if (tk >= left) st[n][0] = st[n][1] = -INFINITY;
-              if (tk + 8 >= left) st[n][2] = st[n][3] = -INFINITY;
-            }
-            raise |= fmaxf(st[n][0], st[n][2]) > m[hp][n][0] + 8.f || fmaxf(st[n][1], st[n][3]) > m[hp][n][1] + 8.f;
-          }
-          // The maximum moves only when a score passes it by more than 2^8: weights stay
-          // below 2^8 (a half holds 2^16), and most tiles rescale nothing.
-          if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                float mx = fmaxf(st[n][k], st[n][k + 2]);
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                mx = fmaxf(m[hp][n][k], mx);
-                const float c = mx == -INFINITY ? 1.f : ptx::ex2(m[hp][n][k] - mx);
-                m[hp][n][k] = mx;
-                l[hp][n][k] *= c;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                  o[hp][n][i][k] *= c;
-                  o[hp][n][i][k + 2] *= c;
-                }
-              }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float pr[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) pr[k] = ptx::ex2(st[n][k] - m[hp][n][k & 1]);
-            l[hp][n][0] += pr[0] + pr[2];
-            l[hp][n][1] += pr[1] + pr[3];
-            pb[n][0] = q8::transpose8x8(DT<__half>::pack2(pr[0], pr[1]));
-            pb[n][1] = q8::transpose8x8(DT<__half>::pack2(pr[2], pr[3]));
-          }
-          // ---- O^T += v_scale (V^T P^T); lane (g, tig): D / 8 bytes of tokens tv0, tv1 and those + 8
-          constexpr int VW = D / 32;  // 32-bit words of a token
-          uint32_t v[4][VW];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int t = (k & 1 ? tv1 : tv0);
-            const uint8_t* src = vp + row_off<ROWB>(t, hp * D + g * (D / 8)) + (k >> 1) * 8 * ROWB;
-            if constexpr (VW == 4) {
-              const uint4 u = *reinterpret_cast<const uint4*>(src);
-              v[k][0] = u.x, v[k][1] = u.y, v[k][2] = u.z, v[k][3] = u.w;
-            } else if constexpr (VW == 2) {
-              const uint2 u = *reinterpret_cast<const uint2*>(src);
-              v[k][0] = u.x, v[k][1] = u.y;
-            } else {
-              v[k][0] = *reinterpret_cast<const uint32_t*>(src);
-            }
-            if (partial && t + (k >> 1) * 8 >= left) {  // what lies behind the context may be NaN
-#pragma unroll
-              for (int x = 0; x < VW; ++x) v[k][x] = 0u;
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < VW; ++x)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t sel = half ? 0x7362 : 0x5140;
-              const uint32_t lo = __byte_perm(v[0][x], v[1][x], sel), hi = __byte_perm(v[2][x], v[3][x], sel);
-              const uint32_t a0 = q8::decode2(lo), a1 = q8::decode2(lo >> 16);
-              const uint32_t a2 = q8::decode2(hi), a3 = q8::decode2(hi >> 16);
-              const int i = x * 2 + half;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (BS8) {
-                  float acc1[4] = {0.f, 0.f, 0.f, 0.f};
-                  q8::mma8(acc, a0, a1, pb[n][0]);
-                  q8::mma8(acc1, a2, a3, pb[n][1]);
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) o[hp][n][i][k] = fmaf(vs1, acc1[k], o[hp][n][i][k]);
-                } else {
-                  q8::mma16(acc, a0, a1, a2, a3, pb[n][0], pb[n][1]);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[hp][n][i][k] = fmaf(vs0, acc[k], o[hp][n][i][k]);
-              }
-            }
         }
+        umma::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&p_full[b]);
+        ++it;
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&empty_bar[stage]);
-      if (++stage == NS) {
-        stage = 0;
-        phase ^= 1;
-      }
-    }
 
-    // ---------------- the share's end: merge the four warps ----------------
-    ptx::named_barrier_sync(1, 128);  // all have read the previous merge
+      // ---------------- the share's end ----------------
 #pragma unroll
-    for (int hp = 0; hp < HP; ++hp)
+      for (int i = 0; i < HG; ++i) {
+        float sum = l[i];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) red_s[wq * 16 + i] = sum;
+      }
+      wait(&p_empty[(it - 1) & 1], ((it - 1) >> 1) & 1);
+      umma::fence_after_sync();
+      float o[GP], o1[GP], o2[GP];
+      {
+        const uint32_t at = lane_addr + L::kOCol + my_hp * GP;
+        umma::ld_32x32b<GP>(at, o);
+        umma::ld_32x32b<GP>(at + HG, o1);
+        umma::ld_32x32b<GP>(at + 2 * HG, o2);
+        umma::ld_wait();
+      }
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(o_empty);
+      ++share;
+      ptx::named_barrier_sync(1, 128);
+      const int r0 = my_hp * GP;
+      float* part = cur.n_parts == 1 ? nullptr : part_slot(p, blockIdx.x, (int)blockIdx.x == cur.first_cta);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float sum = l[hp][n][k];
+      for (int h = 0; h < GP; ++h) {
+        if (h >= nh || !mine) continue;
+        const float M = M_s[r0 + h];
+        const float A = (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * (M == -INFINITY ? 0.f : ptx::ex2(M - R_s[r0 + h]));
+        float Ls = 0.f;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          const int head = n * 8 + tig * 2 + k;
-          if (head >= G) continue;
-          const int r = warp * R + hp * G + head;
-          if (g == 0) {
-            cm[r] = m[hp][n][k];
-            cl[r] = sum;
+        for (int k = 0; k < 4; ++k) Ls += red_s[k * 16 + r0 + h];
+        if (!part) {
+          out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(A / Ls);
+        } else {
+          __stcg(part + (r0 + h) * D + dim, A);
+          if (dim == 0) __stcg(reinterpret_cast<float2*>(part + HG * D + (r0 + h) * 2), make_float2(R_s[r0 + h], Ls));
+        }
+      }
+      if (part) {
+        auto sync = [] { ptx::named_barrier_sync(1, 128); };
+        if (last_to_arrive(p, cur, cur.b * units + cur.h, flag, tid, sync)) {
+          // All parts' (R, sum) at once: 8 threads a row; then the rows' weighted sums.  The weight
+          // buffers are free (their products are done): they take a factor per part and row.
+          float* f = reinterpret_cast<float*>(base + L::kPOff);
+          constexpr int kAtOnce = 2 * L::kP / 4 / HG;
+          float acc[GP];
+          const int row = tid >> 3;
+          const bool has = row < HG && row % GP < nh && pair * HP + row / GP < Hkv;
+          float M = -INFINITY, Ls = 0.f;
+          for (int c = tid & 7; has && c < cur.n_parts; c += 8)
+            M = fmaxf(M, __ldcg(part_slot(p, cur.first_cta + c, c == 0) + HG * D + row * 2));
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+#pragma unroll
+          for (int h = 0; h < GP; ++h) acc[h] = 0.f;
+          for (int c0 = 0; c0 < cur.n_parts; c0 += kAtOnce) {
+            const int c1 = min(cur.n_parts, c0 + kAtOnce);
+            for (int c = c0 + (tid & 7); has && c < c1; c += 8) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_slot(p, cur.first_cta + c, c == 0) + HG * D + row * 2));
+              const float e = exp2f(ml.x - M);
+              f[(c - c0) * HG + row] = e;
+              Ls = fmaf(ml.y, e, Ls);
+            }
+            sync();
+            if (mine) {
+#pragma unroll 4
+              for (int c = c0; c < c1; ++c) {
+                const float* src = part_slot(p, cur.first_cta + c, c == 0) + r0 * D + dim;
+#pragma unroll
+                for (int h = 0; h < GP; ++h)
+                  if (h < nh) acc[h] = fmaf(__ldcg(src + h * D), f[(c - c0) * HG + r0 + h], acc[h]);
+              }
+            }
+            sync();
           }
-          float2* dst = reinterpret_cast<float2*>(co + (size_t)r * D + g * (D / 8));
 #pragma unroll
-          for (int i = 0; i < KS; ++i) dst[i] = make_float2(o[hp][n][i][k], o[hp][n][i][k + 2]);
-        }
-    ptx::named_barrier_sync(1, 128);
-    T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * R) * D;
-    float* mine = s.n_parts == 1 ? nullptr : part_slot(p, blockIdx.x, (int)blockIdx.x == s.first_cta);
-    for (int i = threadIdx.x; i < R * D; i += 128) {
-      const int r = i / D;
-      float M = cm[r];
+          for (int d = 1; d < 8; d <<= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, d);
+          if (has && (tid & 7) == 0) red_s[row] = Ls;
+          sync();
 #pragma unroll
-      for (int x = 1; x < 4; ++x) M = fmaxf(M, cm[x * R + r]);
-      float Lsum = 0.f, A = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        // a warp without tokens in this share has m = -inf and adds nothing
-        const float e = cm[x * R + r] == -INFINITY ? 0.f : ptx::ex2(cm[x * R + r] - M);
-        Lsum = fmaf(cl[x * R + r], e, Lsum);
-        A = fmaf(co[(size_t)x * R * D + i], e, A);
-      }
-      if (!mine) {
-        out[i] = DT<T>::from_f(A / Lsum);
-      } else {
-        __stcg(mine + i, A);
-        if (i % D == 0) {
-          __stcg(mine + R * D + r * 2, M);
-          __stcg(mine + R * D + r * 2 + 1, Lsum);
+          for (int h = 0; h < GP; ++h)
+            if (mine && h < nh) out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(acc[h] / red_s[r0 + h]);
         }
       }
+      ptx::named_barrier_sync(1, 128);  // red_s, M_s and R_s have been read
     }
-    if (mine)
-      join_parts<T, D, 128>(p, s, s.b * heads + s.h, R, s.h * R, flag, threadIdx.x, [] { ptx::named_barrier_sync(1, 128); });
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    umma::fence_after_sync();
+    umma::tmem_dealloc(tmem, L::kTmemCols);
   }
 }
 
 template <typename T>
 int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
-  const long long most = (long long)p.batch * p.n_kv_heads * ((p.max_ctx_tokens + kTile - 1) / kTile + kUnitTiles);
+  const long long most = (long long)p.batch * p.n_kv_heads * (tiles_of(p.max_ctx_tokens, kSimtTile) + kUnitTiles);
   const long long pieces = (most + kMinPiece - 1) / kMinPiece;
   const int grid = (int)(pieces < kMaxCtas ? pieces : kMaxCtas);
   switch (head_dim) {
@@ -773,77 +972,64 @@ int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
   return TVK_OK;
 }
 
-constexpr int kSmemPerCta = 112 * 1024;  // two CTAs on an SM
 
-template <typename T, int D, int HP, int NT, bool BS8>
-int launch_tc(Q8Params p, cudaStream_t stream) {
-  using L = TcLayout<D, HP>;
+template <typename T, int D, int GP>
+int launch_tc(const Q8Params& p, cudaStream_t stream) {
+  using L = TcLayout<D, GP>;
   tvk::EncodeTiledFn encode = tvk::encode_tiled_fn();
   if (!encode) {
     tvk::set_error("cuTensorMapEncodeTiled is not available from the driver");
     return TVK_ERR_CUDA;
   }
+  // A row of the box is 128 bytes: HP heads, of which the last may lie beyond the tensor and read as zeros.
   const cuuint64_t row = (cuuint64_t)p.n_kv_heads * D;
   const cuuint64_t dims[3] = {row, (cuuint64_t)p.block_size, (cuuint64_t)p.num_blocks};
   const cuuint64_t strides[2] = {row, row * p.block_size};
-  const cuuint32_t box[3] = {(cuuint32_t)L::ROWB, (cuuint32_t)(p.block_size < kTile ? p.block_size : kTile), 1u};
+  const cuuint32_t box[3] = {128u, (cuuint32_t)(p.block_size < kTcTile ? p.block_size : kTcTile), 1u};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
-  const CUtensorMapSwizzle sw = L::ROWB == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                : L::ROWB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                : CU_TENSOR_MAP_SWIZZLE_32B;
   CUtensorMap tm[2];
   for (int i = 0; i < 2; ++i) {
     const CUresult r = encode(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(i ? p.v_cache : p.k_cache), dims,
-                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
       tvk::set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
       return TVK_ERR_CUDA;
     }
   }
-  // as many stages as fit twice on an SM, 8 at most
-  p.n_stages = 2;
-  while (p.n_stages < 8 && L::bytes(p.n_stages + 1, p.group) <= kSmemPerCta) ++p.n_stages;
-  const int smem = L::bytes(p.n_stages, p.group);
-  auto kern = paged_decode_q8_tc_kernel<T, D, HP, NT, BS8>;
+  auto kern = paged_decode_q8_tc_kernel<T, D, GP>;
   int dev = 0;
   TVK_CHECK_CUDA(cudaGetDevice(&dev));
   static std::atomic<unsigned long long> attr_set{0};  // one bit per device
   if (dev >= 64 || !(attr_set.load() >> dev & 1)) {
-    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerCta));
+    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
     if (dev < 64) attr_set.fetch_or(1ull << dev);
   }
-  const long long most =
-      (long long)p.batch * (p.n_kv_heads / HP) * ((p.max_ctx_tokens + kTile - 1) / kTile + kUnitTiles);
+  const int units = (p.n_kv_heads + L::HP - 1) / L::HP * ((p.group + GP - 1) / GP);
+  const long long most = (long long)p.batch * units * (tiles_of(p.max_ctx_tokens, kTcTile) + kUnitTiles);
   const long long pieces = (most + kMinPiece - 1) / kMinPiece;
   const int grid = (int)(pieces < kTcCtas ? pieces : kTcCtas);
-  TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, kTcThreads, smem, stream, p, tm[0], tm[1]));
+  TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, kTcThreads, L::kBytes, stream, p, tm[0], tm[1]));
   TVK_CHECK_LAUNCH("paged_decode_q8_tc");
   return TVK_OK;
 }
 
-template <typename T, int D, int HP>
-int launch_heads(const Q8Params& p, cudaStream_t stream) {
-  const bool bs8 = p.block_size == 8;
-  if (p.group <= 8) return bs8 ? launch_tc<T, D, HP, 1, true>(p, stream) : launch_tc<T, D, HP, 1, false>(p, stream);
-  return bs8 ? launch_tc<T, D, HP, 2, true>(p, stream) : launch_tc<T, D, HP, 2, false>(p, stream);
-}
-
-// 16-bit queries on the tensor cores where 64-token tiles are whole blocks or lie in one.
+// 16-bit queries on the tensor cores where 128-token tiles are whole blocks or lie in one.
+// Query heads per unit: as few as hold the group, but no more than 16 over the HP KV heads.
 template <typename T>
 int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
   const int bs = p.block_size;
-  if (!(bs == 8 || bs == 16 || bs == 32 || bs % kTile == 0)) return launch_simt<T>(p, head_dim, stream);
-  if (head_dim == 128) return launch_heads<T, 128, 1>(p, stream);
-  if (head_dim == 64)
-    return p.n_kv_heads % 2 == 0 ? launch_heads<T, 64, 2>(p, stream) : launch_heads<T, 64, 1>(p, stream);
-  return p.n_kv_heads % 4 == 0 ? launch_heads<T, 32, 4>(p, stream) : launch_heads<T, 32, 1>(p, stream);
+  if (!(bs == 8 || bs == 16 || bs == 32 || bs == 64 || bs % kTcTile == 0)) return launch_simt<T>(p, head_dim, stream);
+  if (head_dim == 32) return launch_tc<T, 32, 4>(p, stream);
+  if (head_dim == 64) return p.group <= 4 ? launch_tc<T, 64, 4>(p, stream) : launch_tc<T, 64, 8>(p, stream);
+  return p.group <= 4 ? launch_tc<T, 128, 4>(p, stream)
+                      : p.group <= 8 ? launch_tc<T, 128, 8>(p, stream) : launch_tc<T, 128, 16>(p, stream);
 }
 
 }  // namespace
 
 extern "C" size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads) {
-  size_t units = batch > 0 && n_kv_heads > 0 ? (size_t)batch * n_kv_heads : 0;
+  const size_t units = batch > 0 && n_kv_heads > 0 ? (size_t)batch * n_kv_heads * kMaxParts : 0;
   return tvk::kWorkspaceHeader + (size_t)2 * kMaxCtas * kSlotFloats * sizeof(float) + units * sizeof(int);
 }
 
@@ -861,7 +1047,7 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
   TVK_CHECK_ARG(block_size > 0 && num_blocks > 0 && max_blocks > 0,
                 "block_size, num_blocks and max_blocks must be positive");
   TVK_CHECK_ARG((long long)max_blocks * block_size < 0x7fffffffLL, "a table spans more than 2^31 tokens");
-  TVK_CHECK_ARG((long long)batch * n_kv_heads * ((long long)max_blocks * block_size / kTile + 1 + kUnitTiles) < 0x7fffffffLL,
+  TVK_CHECK_ARG((long long)batch * n_kv_heads * ((long long)max_blocks * block_size / kSimtTile + 1 + kUnitTiles) < 0x7fffffffLL,
                 "batch x KV heads x table tiles exceeds the 32-bit work index");
   TVK_CHECK_ARG(dtype == TVK_DTYPE_F32 || dtype == TVK_DTYPE_F16 || dtype == TVK_DTYPE_BF16, "unknown dtype %d", dtype);
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) {
