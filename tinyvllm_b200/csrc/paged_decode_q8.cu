@@ -31,7 +31,7 @@ constexpr int kMaxGroup = 16;        // query heads per KV head
 constexpr int kMaxCtas = 592;        // pieces a call is cut into at most (simt: four CTAs on each of 148 SMs)
 constexpr int kTcCtas = 296;         // tensor-core kernel: two CTAs on each SM
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
-constexpr int kMinPiece = 2;         // shortest piece, in tiles
+constexpr int kMinPiece = 1;         // shortest piece, in tiles
 constexpr int kMaxParts = 4;         // units per (sequence, KV head) at most, see group_splits
 constexpr int kSlotFloats = 2240;    // partials of one cut unit: rows * (D + 2), at most 64 * 34, 32 * 66 or 16 * 130
 
@@ -426,6 +426,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsign
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, limit_ns));
 }
 
+// One byte to shared memory.  No memory clobber, so that the loads of the next head may pass it: for
+// bytes that only the matrix unit reads, after a proxy fence (which is ordered behind it).
+__device__ __forceinline__ void store_byte(uint32_t addr, uint32_t x) {
+  asm volatile("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tst.shared.u8 [%0], h;\n\t}" ::"r"(addr), "r"(x));
+}
+
 // Largest value of a warp (NaN only where all are).
 __device__ __forceinline__ float warp_max(float x) {
   float r;
@@ -455,14 +461,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   uint64_t* q_empty = q_full + 2;            // [QB] the share's S^T all done, query factors read
   uint64_t* o_empty = q_empty + 2;           // O^T read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
-  // misc: query factors [2][16], warp results [4][16][2], per head M, R, two factors [4][16], a flag
-  float* hs_s = reinterpret_cast<float*>(base + L::kMiscOff);
+  // misc: per head {limit of s + log2 v_scale, limit of s, M, R}, query factors [2][16], warp results
+  // [4][16][2], two factors per head [16][2], a flag
+  float4* ref_s = reinterpret_cast<float4*>(base + L::kMiscOff);
+  float* hs_s = reinterpret_cast<float*>(ref_s + 16);
   float* red_s = hs_s + 32;
-  float* M_s = red_s + 128;
-  float* R_s = M_s + 16;
-  float* c_s = R_s + 16;
-  float* lc_s = c_s + 16;
-  int* flag = reinterpret_cast<int*>(lc_s + 16);
+  float2* c_s = reinterpret_cast<float2*>(red_s + 128);
+  int* flag = reinterpret_cast<int*>(c_s + 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -586,58 +591,80 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     constexpr uint32_t idesc_s = umma::idesc_e4m3(128, L::NS, false);
     constexpr uint32_t idesc_o = umma::idesc_e4m3(128, L::NO, true);
     uint32_t it = 0, share = 0;
-    bool prev_first = false, ok = true;
-    // P.V of tile t, its V at place n, share sh
-    auto issue_pv = [&](uint32_t t, uint32_t n, bool first_of_share, uint32_t sh) {
-      const uint32_t b = t & 1, sl = slot_of(n);
-      ok = ok && warp_wait(&full_bar[sl], round_of(n), p.wait_ns);
-      if (first_of_share) ok = ok && warp_wait(o_empty, (sh & 1) ^ 1, p.wait_ns);
-      ok = ok && warp_wait(&p_full[b], (t >> 1) & 1, p.wait_ns);
-      if (!ok) return;
+    bool ok = true;
+    // The P.V that is due: tile, place of its V, whether it starts its share, the share.
+    bool due = false, due_first = false;
+    uint32_t due_tile = 0, due_at = 0, due_share = 0;
+    auto pv_ready = [&]() -> bool {
+      return __all_sync(0xffffffffu, ptx::mbar_test(&p_full[due_tile & 1], (due_tile >> 1) & 1) &&
+                                         ptx::mbar_test(&full_bar[slot_of(due_at)], round_of(due_at)) &&
+                                         (!due_first || ptx::mbar_test(o_empty, (due_share & 1) ^ 1)));
+    };
+    auto issue_pv = [&]() {
+      const uint32_t b = due_tile & 1, sl = slot_of(due_at);
       umma::fence_after_sync();
       if (lane == 0) {
         const uint32_t va = base_u32 + sl * L::kSlot, pa = base_u32 + L::kPOff + b * L::kP;
 #pragma unroll
         for (int k = 0; k < kTcTile / 32; ++k)
           umma::mma_f8_ss(tmem + L::kOCol, umma::smem_desc_sw128(va + k * 32 * 128, 0, 1024),
-                          umma::smem_desc_sw128(pa + k * 32, 0, 1024), idesc_o, !(first_of_share && k == 0));
+                          umma::smem_desc_sw128(pa + k * 32, 0, 1024), idesc_o, !(due_first && k == 0));
         umma::commit(&empty_bar[sl]);
         umma::commit(&p_empty[b]);
       }
       __syncwarp();
+      due = false;
     };
     while (ok && w.next(p, s)) {
       if (s.tok0 == s.tok1) continue;
       const uint32_t qb = share % QB;
       for (int t0 = s.tok0; ok && t0 < s.tok1; t0 += kTcTile) {
+        // S^T of this tile and P.V of the one before, whichever can go first.
         const uint32_t b = it & 1, n = k_at(it), sl = slot_of(n);
-        if (t0 == s.tok0) ok = ok && warp_wait(&q_full[qb], (share / QB) & 1, p.wait_ns);
-        ok = ok && warp_wait(&s_empty[b], ((it >> 1) & 1) ^ 1, p.wait_ns);
-        ok = ok && warp_wait(&full_bar[sl], round_of(n), p.wait_ns);
-        if (!ok) break;
-        umma::fence_after_sync();
-        if (lane == 0) {
-          const uint32_t ka = base_u32 + sl * L::kSlot, qa = base_u32 + L::kQOff + qb * L::kQ;
+        bool scored = false;
+        const uint64_t since = ptx::globaltimer();
+        while (!scored || due) {
+          if (!scored &&
+              __all_sync(0xffffffffu, ptx::mbar_test(&full_bar[sl], round_of(n)) &&
+                                          ptx::mbar_test(&s_empty[b], ((it >> 1) & 1) ^ 1) &&
+                                          (t0 != s.tok0 || ptx::mbar_test(&q_full[qb], (share / QB) & 1)))) {
+            umma::fence_after_sync();
+            if (lane == 0) {
+              const uint32_t ka = base_u32 + sl * L::kSlot, qa = base_u32 + L::kQOff + qb * L::kQ;
 #pragma unroll
-          for (int hp = 0; hp < HP; ++hp)
+              for (int hp = 0; hp < HP; ++hp)
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k)
-              umma::mma_f8_ss(tmem + (b * HP + hp) * L::NS, umma::smem_desc_sw128(ka + hp * D + k * 32, 0, 1024),
-                              umma::smem_desc_sw128(qa + hp * L::NS * 128 + k * 32, 0, 1024), idesc_s, k > 0);
-          umma::commit(&s_full[b]);
-          umma::commit(&empty_bar[sl]);
-          if (t0 + kTcTile >= s.tok1) umma::commit(&q_empty[qb]);
+                for (int k = 0; k < D / 32; ++k)
+                  umma::mma_f8_ss(tmem + (b * HP + hp) * L::NS, umma::smem_desc_sw128(ka + hp * D + k * 32, 0, 1024),
+                                  umma::smem_desc_sw128(qa + hp * L::NS * 128 + k * 32, 0, 1024), idesc_s, k > 0);
+              umma::commit(&s_full[b]);
+              umma::commit(&empty_bar[sl]);
+              if (t0 + kTcTile >= s.tok1) umma::commit(&q_empty[qb]);
+            }
+            __syncwarp();
+            scored = true;
+          }
+          if (due && pv_ready()) issue_pv();
+          if ((!scored || due) && __any_sync(0xffffffffu, ptx::globaltimer() - since > p.wait_ns)) {
+            ok = false;
+            break;
+          }
         }
-        __syncwarp();
-        if (it > 0) issue_pv(it - 1, v_at(it - 1), prev_first, t0 == s.tok0 ? share - 1 : share);
-        prev_first = t0 == s.tok0;
+        due = ok;
+        due_tile = it;
+        due_at = v_at(it);
+        due_first = t0 == s.tok0;
+        due_share = share;
         ++it;
       }
       ++share;
     }
-    if (ok && it > 0) {
-      issue_pv(it - 1, v_at(it - 1) - 1, prev_first, share - 1);
-      ok = ok && warp_wait(&p_empty[(it - 1) & 1], ((it - 1) >> 1) & 1, p.wait_ns);  // nothing runs when TMEM is freed
+    if (ok && due) {
+      --due_at;  // no K behind the last tile
+      const uint64_t since = ptx::globaltimer();
+      while (!pv_ready() && ok) ok = !__any_sync(0xffffffffu, ptx::globaltimer() - since > p.wait_ns);
+      if (ok) issue_pv();
+      ok = ok && warp_wait(&p_empty[due_tile & 1], (due_tile >> 1) & 1, p.wait_ns);  // nothing runs when TMEM is freed
     }
     if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
   } else if (warp == 2) {
@@ -728,7 +755,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const int head0 = (pair * HP + my_hp) * G + g0;  // this thread's first output head
       const bool mine = pair * HP + my_hp < Hkv;
       const uint32_t qb = share % QB;
-      if (tid < 16) M_s[tid] = R_s[tid] = -INFINITY;
+      if (tid < HG) {  // heads beyond the group never ask for new references
+        const float lim = tid % GP < nh ? -INFINITY : INFINITY;
+        ref_s[tid] = make_float4(lim, lim, -INFINITY, -INFINITY);
+      }
       wait(&q_full[qb], (share / QB) & 1);
       float hs[HG], l[HG];
 #pragma unroll
@@ -738,7 +768,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&q_empty[qb]);
-      ptx::named_barrier_sync(1, 128);  // M_s and R_s are set
+      ptx::named_barrier_sync(1, 128);  // the references are set
 
       for (int t0 = cur.tok0; t0 < cur.tok1; t0 += kTcTile) {
         const uint32_t b = it & 1;
@@ -769,7 +799,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             const int i = hp * GP + h;
             const float sum = fmaf(c3[h], kLowPart, c2[h] + c1[h]) + c0[h];
             x[i] = live ? sum * (ks[hp] * hs[i]) : -INFINITY;
-            if (h < nh) raise |= x[i] + lv[hp] > M_s[i] + 8.f || x[i] > R_s[i] + 64.f;
+            const float2 lim = *reinterpret_cast<const float2*>(&ref_s[i]);
+            raise |= (x[i] + lv[hp] > lim.x) | (x[i] > lim.y);
           }
         }
         umma::fence_before_sync();
@@ -784,22 +815,23 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           }
           ptx::named_barrier_sync(1, 128);
           if (tid < HG) {
-            float nm = M_s[tid], nr = R_s[tid];
+            const float4 was = ref_s[tid];
+            float nm = was.z, nr = was.w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              nm = fmaxf(nm, red_s[(k * 16 + tid) * 2] - 4.f);
-              nr = fmaxf(nr, red_s[(k * 16 + tid) * 2 + 1]);
+              const float2 top = *reinterpret_cast<const float2*>(red_s + (k * 16 + tid) * 2);
+              nm = fmaxf(nm, top.x - 4.f);
+              nr = fmaxf(nr, top.y);
             }
-            c_s[tid] = nm == -INFINITY ? 1.f : ptx::ex2(M_s[tid] - nm);
-            lc_s[tid] = nr == -INFINITY ? 1.f : ptx::ex2(R_s[tid] - nr);
-            M_s[tid] = nm;
-            R_s[tid] = nr;
+            c_s[tid] = make_float2(nm == -INFINITY ? 1.f : ptx::ex2(was.z - nm), nr == -INFINITY ? 1.f : ptx::ex2(was.w - nr));
+            const bool used = tid % GP < nh;
+            ref_s[tid] = make_float4(used ? nm + 8.f : INFINITY, used ? nr + 64.f : INFINITY, nm, nr);
           }
           if (t0 != cur.tok0) wait(&p_empty[b ^ 1], ((it - 1) >> 1) & 1);  // P.V of the tile before: O^T is at rest
           ptx::named_barrier_sync(1, 128);
           umma::fence_after_sync();
 #pragma unroll
-          for (int i = 0; i < HG; ++i) l[i] *= lc_s[i];
+          for (int i = 0; i < HG; ++i) l[i] *= c_s[i].y;
           if (t0 != cur.tok0) {
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
@@ -808,7 +840,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
               umma::ld_32x32b<GP>(at, o);
               umma::ld_wait();
 #pragma unroll
-              for (int h = 0; h < GP; ++h) o[h] *= c_s[my_hp * GP + h];
+              for (int h = 0; h < GP; ++h) o[h] *= c_s[my_hp * GP + h].x;
               umma::st_32x32b<GP>(at, o);
             }
             umma::st_wait();
@@ -817,19 +849,18 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         }
         // Weights, their sums, and their parts as rows of P^T: this thread's token is byte tid.
         wait(&p_empty[b], ((it >> 1) & 1) ^ 1);
-        uint8_t* pw = base + L::kPOff + b * L::kP;
+        const uint32_t pw = base_u32 + L::kPOff + b * L::kP + tid;
 #pragma unroll
         for (int hp = 0; hp < HP; ++hp)
 #pragma unroll
-          for (int h = 0; h < GP; h += 2) {
-            if (h >= nh) continue;
+          for (int h = 0; h < GP; h += 2) {  // heads beyond the group too: a branch would cost more
             float wt[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int i = hp * GP + h + k;
-              const float M = M_s[i];
-              l[i] += ptx::ex2(x[i] - R_s[i]);
-              wt[k] = ptx::ex2(x[i] + lv[hp] - (M == -INFINITY ? 0.f : M));
+              const float2 ref = *reinterpret_cast<const float2*>(&ref_s[i].z);
+              l[i] += ptx::ex2(x[i] - ref.y);
+              wt[k] = ptx::ex2(x[i] + lv[hp] - (ref.x == -INFINITY ? 0.f : ref.x));
             }
             const uint32_t hw = DT<__half>::pack2(wt[0], wt[1]);
             const uint32_t c1 = q8::encode2h(hw), r1 = q8::sub2h(hw, q8::decode2h(c1));
@@ -839,9 +870,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             const uint32_t cs[3] = {c1, c2, c3};
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
+              // swz128(row, tid): the row's part of the swizzle is an exclusive or of constants
               const int row = k * HG + hp * GP + h;
-              pw[swz128(row, tid)] = (uint8_t)cs[k];
-              if (h + 1 < nh) pw[swz128(row + 1, tid)] = (uint8_t)(cs[k] >> 8);
+              store_byte((pw ^ ((row & 7) << 4)) + row * 128, cs[k]);
+              store_byte((pw ^ (((row + 1) & 7) << 4)) + (row + 1) * 128, cs[k] >> 8);
             }
           }
         // What lies behind the context has no weight, but may be NaN: zeros for V.
@@ -889,8 +921,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
         if (h >= nh || !mine) continue;
-        const float M = M_s[r0 + h];
-        const float A = (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * (M == -INFINITY ? 0.f : ptx::ex2(M - R_s[r0 + h]));
+        const float2 ref = *reinterpret_cast<const float2*>(&ref_s[r0 + h].z);
+        const float A = (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * (ref.x == -INFINITY ? 0.f : ptx::ex2(ref.x - ref.y));
         float Ls = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) Ls += red_s[k * 16 + r0 + h];
@@ -898,7 +930,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(A / Ls);
         } else {
           __stcg(part + (r0 + h) * D + dim, A);
-          if (dim == 0) __stcg(reinterpret_cast<float2*>(part + HG * D + (r0 + h) * 2), make_float2(R_s[r0 + h], Ls));
+          if (dim == 0) __stcg(reinterpret_cast<float2*>(part + HG * D + (r0 + h) * 2), make_float2(ref.y, Ls));
         }
       }
       if (part) {
@@ -947,7 +979,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             if (mine && h < nh) out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(acc[h] / red_s[r0 + h]);
         }
       }
-      ptx::named_barrier_sync(1, 128);  // red_s, M_s and R_s have been read
+      ptx::named_barrier_sync(1, 128);  // red_s and ref_s have been read
     }
   }
   umma::fence_before_sync();
