@@ -8,13 +8,16 @@
 // a block's v_scale goes into the weights of its tokens, both in fp32.
 //
 // Work split.  The live tokens of all (sequence, KV head) units are laid out on
-// one line in tiles of tokens (plus a few tiles' worth per unit for its start and
-// end) and cut into equal pieces, one per CTA; heads of a sequence lie next
-// to each other.  Every CTA works its piece out of the context lengths alone.  A
-// unit that lies in one piece is written at once; one cut by a border leaves fp32
-// partials (max, sum, unnormalised output) in the workspace, and the CTA that
-// arrives last at the unit's counter adds them up in CTA order, so the result does
-// not depend on who that is.  Nobody waits for anybody.
+// one line in tiles of tokens (plus two tiles' worth per unit for its start and
+// end), heads of a sequence next to each other, and cut into equal pieces, one per CTA,
+// which every CTA works out from the context lengths alone.  A unit of few tiles
+// belongs whole to the piece that it starts in.  A longer one that a border cuts
+// leaves fp32 partials (max, sum, unnormalised output) by piece in the workspace, and
+// the CTA that arrives last at the unit's counter adds them up in piece order, so the
+// result does not depend on who that is.  Nobody waits for anybody.  (Leaving the
+// line's last fifth to the CTAs that are done first, in smaller pieces by ticket, was
+// no gain: 256 sequences of 128-4096 tokens 229 us instead of 208, long ones 82 instead of 57,
+// for the joins of many parts.)
 #include <math.h>
 
 #include <atomic>
@@ -26,13 +29,15 @@
 namespace {
 
 constexpr int kSimtTile = 32;        // tokens the simt kernel stages at a time, and its tile of the work line
+constexpr int kSimtWhole = 2;        // its units of up to so many tiles are not cut
 constexpr int kTcTile = 128;         // the same for the tensor-core kernel: the rows of a matrix instruction
+constexpr int kTcWhole = 6;          // joining parts costs as much as 4 to 5 tiles in a row
 constexpr int kMaxGroup = 16;        // query heads per KV head
-constexpr int kMaxCtas = 592;        // pieces a call is cut into at most (simt: four CTAs on each of 148 SMs)
-constexpr int kTcCtas = 296;         // tensor-core kernel: two CTAs on each SM
+constexpr int kSimtCtas = 592;       // four CTAs on each of 148 SMs
+constexpr int kTcCtas = 296;         // two CTAs on each SM
+constexpr int kMaxPieces = kSimtCtas;
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
-constexpr int kMinPiece = 1;         // shortest piece, in tiles
-constexpr int kMaxParts = 4;         // units per (sequence, KV head) at most, see group_splits
+constexpr int kMaxParts = 4;         // units per (sequence, KV head) at most, where groups are split
 constexpr int kSlotFloats = 2240;    // partials of one cut unit: rows * (D + 2), at most 64 * 34, 32 * 66 or 16 * 130
 
 struct Q8Params {
@@ -43,10 +48,11 @@ struct Q8Params {
   const uint8_t *k_cache, *v_cache;
   const float *k_scale, *v_scale;
   int* status;
-  float* part;     // [2 * kMaxCtas][kSlotFloats]
+  float* part;     // [2 * kMaxPieces][kSlotFloats]
   int* counters;   // [batch * n_kv_heads * kMaxParts], zero between calls
   int batch, n_heads, n_kv_heads, group, block_size, num_blocks, max_blocks;
   int max_ctx_tokens;
+  int team;                    // tensor-core kernel: CTAs that walk one piece, each its own unit of every group
   float scale_log2;            // log2(e) / sqrt(head_dim)
   int n_stages;                // ring depth of the tensor-core kernel
   unsigned long long wait_ns;  // wall-time limit of every mbarrier wait
@@ -59,38 +65,52 @@ __device__ __forceinline__ int effective_ctx(const Q8Params& p, int b) {
 }
 __host__ __device__ __forceinline__ int tiles_of(int ctx, int tile) { return (ctx + tile - 1) / tile; }
 
-// One CTA's share of one unit: tokens [tok0, tok1) of (b, h).  A unit without
-// context is one share with tok0 == tok1 and n_parts 1.
+// One piece's share of one unit: tokens [tok0, tok1) of (b, h).  A unit without
+// context is one share with tok0 == tok1.
 struct Share {
   int b, h, ctx, tok0, tok1;
-  int n_parts;    // CTAs that share the unit
-  int first_cta;  // the first of them
+  int piece;
+  int n_parts;      // pieces that share the unit
+  int first_piece;  // the first of them
 };
 
-// Walks the units of this CTA's piece.  `heads` = units per sequence.  All
-// members are the same in every lane of the calling warp.
-template <int TILE>
-struct Walker {
-  long long x0, x1, total;
-  int pieces, heads;
-  int b, h, ctx;
-  long long at;  // line position where unit (b, h) starts
+// The line and its equal pieces.
+struct Cut {
+  long long total;
+  int pieces;
 
-  // The whole warp calls this.
-  __device__ void start(const Q8Params& p, int heads_, int lane) {
-    heads = heads_;
+  __device__ void make(long long total_, int ctas) {
+    total = total_;
+    pieces = (int)(total < ctas ? total : ctas);
+  }
+  __device__ long long start(int i) const { return total * i / pieces; }
+  __device__ int piece_of(long long x) const { return (int)(((x + 1) * pieces - 1) / total); }
+};
+
+// Walks the units of one piece.  `heads` = units per sequence.  WHOLE: units of up to so
+// many tiles are never cut.
+template <int TILE, int WHOLE>
+struct Walker {
+  long long x0, x1;  // the piece
+  long long at;      // line position where unit (b, h) starts
+  int b, h, ctx, next_ctx, piece;
+
+  // Length of the line; the whole warp calls this.
+  static __device__ long long line(const Q8Params& p, int heads, int lane) {
     long long sum = 0;
     for (int i = lane; i < p.batch; i += 32) sum += tiles_of(effective_ctx(p, i), TILE) + kUnitTiles;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    total = sum * heads;
-    pieces = (int)min((long long)gridDim.x, (total + kMinPiece - 1) / kMinPiece);
-    b = p.batch;
-    if ((int)blockIdx.x >= pieces) return;
-    x0 = total * blockIdx.x / pieces;
-    x1 = total * (blockIdx.x + 1) / pieces;
-    // the sequence that holds x0
+    return sum * heads;
+  }
+
+  // To the unit that holds the start of piece i; the whole warp calls this.
+  __device__ void seek(const Q8Params& p, const Cut& cut, int heads, int i_piece, int lane) {
+    piece = i_piece;
+    x0 = cut.start(i_piece);
+    x1 = cut.start(i_piece + 1);
     long long before = 0;
+    b = p.batch;
     for (int i0 = 0; i0 < p.batch; i0 += 32) {
       const int i = i0 + lane;
       const int c = i < p.batch ? effective_ctx(p, i) : 0;
@@ -111,37 +131,39 @@ struct Walker {
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
+    if (b >= p.batch) return;
     const int w = tiles_of(ctx, TILE) + kUnitTiles;
     h = (int)((x0 - at) / w);
     at += (long long)h * w;
+    next_ctx = b + 1 < p.batch ? effective_ctx(p, b + 1) : 0;
   }
 
-  // The CTA whose piece holds line position x.
-  __device__ int cta_of(long long x) const { return (int)(((x + 1) * pieces - 1) / total); }
-
   // The next share of the piece; false when there is none left.
-  __device__ bool next(const Q8Params& p, Share& s) {
+  __device__ bool next(const Q8Params& p, const Cut& cut, int heads, Share& s) {
     while (b < p.batch && at < x1) {
       const int tiles = tiles_of(ctx, TILE);
-      const long long lo = max(x0 - at, 0LL), hi = min(x1 - at, (long long)tiles);
-      const bool mine = tiles ? lo < hi : lo == 0;
+      long long lo = max(x0 - at, 0LL), hi = min(x1 - at, (long long)tiles);
+      bool mine = lo < hi;
+      s.n_parts = 1;
+      if (tiles <= WHOLE) {
+        mine = lo == 0;  // it starts here
+        hi = tiles;
+      } else if (mine && (lo > 0 || hi < tiles)) {
+        s.first_piece = cut.piece_of(at);
+        s.n_parts = cut.piece_of(at + tiles - 1) - s.first_piece + 1;
+      }
       s.b = b;
       s.h = h;
       s.ctx = ctx;
+      s.piece = piece;
       s.tok0 = (int)lo * TILE;
       s.tok1 = min((int)hi * TILE, ctx);
-      s.first_cta = blockIdx.x;
-      s.n_parts = 1;
-      if (tiles && (lo > 0 || hi < tiles)) {
-        s.first_cta = cta_of(at);
-        s.n_parts = cta_of(at + tiles - 1) - s.first_cta + 1;
-      }
-      if (!tiles) s.tok0 = s.tok1 = 0;
       at += tiles + kUnitTiles;
       if (++h == heads) {
         h = 0;
         ++b;
-        if (b < p.batch) ctx = effective_ctx(p, b);
+        ctx = next_ctx;
+        next_ctx = b + 1 < p.batch ? effective_ctx(p, b + 1) : 0;  // not needed before the next sequence
       }
       if (mine) return true;
     }
@@ -149,11 +171,13 @@ struct Walker {
   }
 };
 
-// Where this CTA leaves its partials of a cut unit.  A CTA is the first of at
-// most one cut unit (the last of its piece) and a later one of at most one (the
-// first of its piece), so two slots do.
+// Where a CTA leaves its partials of a cut unit.  Its piece is the first of at most
+// one cut unit (its last) and a later one of at most one (its first), so two slots do.
 __device__ __forceinline__ float* part_slot(const Q8Params& p, int cta, bool is_first) {
   return p.part + (size_t)(cta * 2 + (is_first ? 1 : 0)) * kSlotFloats;
+}
+__device__ __forceinline__ float* part_of(const Q8Params& p, const Share& s, int c) {
+  return part_slot(p, s.first_piece + c, c == 0);
 }
 
 // Counts the arrival of a share of a cut unit whose partials the calling threads
@@ -177,11 +201,11 @@ __device__ bool last_to_arrive(const Q8Params& p, const Share& s, int unit, int*
 // [n_o] unnormalised sums and then (max, sum) of every row.
 __device__ __forceinline__ float joined(const Q8Params& p, const Share& s, int n_o, int i, int r) {
   float M = -INFINITY;
-  for (int c = 0; c < s.n_parts; ++c) M = fmaxf(M, __ldcg(part_slot(p, s.first_cta + c, c == 0) + n_o + r * 2));
+  for (int c = 0; c < s.n_parts; ++c) M = fmaxf(M, __ldcg(part_of(p, s, c) + n_o + r * 2));
   float L = 0.f, A = 0.f;
 #pragma unroll 4
   for (int c = 0; c < s.n_parts; ++c) {
-    const float* src = part_slot(p, s.first_cta + c, c == 0);
+    const float* src = part_of(p, s, c);
     const float w = exp2f(__ldcg(src + n_o + r * 2) - M);
     L = fmaf(__ldcg(src + n_o + r * 2 + 1), w, L);
     A = fmaf(__ldcg(src + i), w, A);
@@ -206,10 +230,14 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
   __shared__ int flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, bs = p.block_size, Hkv = p.n_kv_heads;
-  Walker<kSimtTile> w;
-  w.start(p, Hkv, lane);
+  using Walk = Walker<kSimtTile, kSimtWhole>;
+  Cut cut;
+  cut.make(Walk::line(p, Hkv, lane), gridDim.x);
+  if ((int)blockIdx.x >= cut.pieces) return;
+  Walk w;
+  w.seek(p, cut, Hkv, blockIdx.x, lane);
   Share s;
-  while (w.next(p, s)) {
+  while (w.next(p, cut, Hkv, s)) {
     T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * G) * D;
     if (s.ctx == 0) {
       for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(0.f);
@@ -314,7 +342,7 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
       for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(qs[i] / lfin[i / D]);
       continue;
     }
-    float* mine = part_slot(p, blockIdx.x, (int)blockIdx.x == s.first_cta);
+    float* mine = part_slot(p, s.piece, s.piece == s.first_piece);
     for (int i = tid; i < G * D; i += 128) __stcg(mine + i, qs[i]);
     for (int i = tid; i < G; i += 128) {
       __stcg(mine + G * D + i * 2, mfin[i]);
@@ -347,8 +375,8 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
 // 256 sequences of 128-4096 tokens, 32/8 heads of 128.  mma.sync on e4m3 itself
 // is converted to halves by the compiler on this architecture and took longer still.)
 //
-// Roles: warp 0 streams K and V tiles (TMA) and their scales (4-byte asynchronous
-// copies); warp 1 issues the products; warp 2 splits the query rows of the next share;
+// Roles: warp 0 streams K tiles (TMA) and their scales (4-byte asynchronous
+// copies), warp 3 V; warp 1 issues the products; warp 2 splits the query rows of the next share;
 // warps 4-7, a thread per token, turn S^T into weights, keep the sums of weights, and
 // at a share's end, a thread per dim, read O^T and write the output.
 // K and V tiles go through one ring of 16 KB slots in the order the products take
@@ -385,7 +413,7 @@ struct TcLayout {
   static constexpr int kBytes = kBarOff + kBars + 1024;
   static_assert(HG <= 16 && kOCol + NO <= 256 && kSlots >= 5 && kSlots <= 7, "sizes");
   static_assert((2 * kSlots + kScaleRing + 14) * 8 <= kBars, "barriers");
-  static_assert(2 * kP / 4 >= HG * kTcCtas / 4, "room for the join's factors, a quarter of the parts at a time");
+  static_assert(2 * kP / 4 >= HG * 8, "room for the join's factors of some parts at a time");
 };
 
 // Byte of row r of a tile with 128-byte rows in the 128-byte swizzle.
@@ -468,6 +496,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   float* red_s = hs_s + 32;
   float2* c_s = reinterpret_cast<float2*>(red_s + 128);
   int* flag = reinterpret_cast<int*>(c_s + 16);
+  Share* cut_s = reinterpret_cast<Share*>(flag + 4);  // [2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -475,7 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       ptx::mbar_init(&full_bar[i], 1);
       ptx::mbar_init(&empty_bar[i], 1);
     }
-    for (int i = 0; i < kScaleRing; ++i) ptx::mbar_init(&sc_full[i], 32);
+    for (int i = 0; i < kScaleRing; ++i) ptx::mbar_init(&sc_full[i], 64);  // every lane of both producers
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&s_full[i], 1);
       ptx::mbar_init(&s_empty[i], 4);
@@ -503,8 +532,19 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   const int rows = p.block_size < kTcTile ? p.block_size : kTcTile;  // rows of one TMA box
   const int nb = kTcTile / rows;                                     // blocks of a tile
   Share s;
-  Walker<kTcTile> w;
-  if (warp != 3) w.start(p, units, lane);
+  using Walk = Walker<kTcTile, kTcWhole>;
+  Cut cut;
+  const int team = p.team, groups = units / team, mate = blockIdx.x % team;  // groups of units per sequence
+  cut.make(Walk::line(p, groups, lane), gridDim.x / team);
+  Walk w;
+  w.b = p.batch;
+  if ((int)blockIdx.x / team < cut.pieces) w.seek(p, cut, groups, blockIdx.x / team, lane);
+  // The next share, with s.h as the unit of this CTA.
+  auto next_share = [&]() -> bool {
+    if (!w.next(p, cut, groups, s)) return false;
+    s.h = s.h * team + mate;
+    return true;
+  };
   // Slot of the n-th tile of the ring's order and the parity of its round.
   auto slot_of = [](uint32_t n) { return n % SL; };
   auto round_of = [](uint32_t n) { return (n / SL) & 1; };
@@ -513,16 +553,19 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   // V(t) follows K(t + 1) if there is one: the last tile's V closes the order.
   auto v_at = [](uint32_t t) { return 2 * t + 2; };
 
-  if (warp == 0) {
-    // ---------------- producer ----------------
-    if (lane == 0) {
-      ptx::prefetch_tmap(&tm_k);
-      ptx::prefetch_tmap(&tm_v);
-    }
+  if (warp == 0 || warp == 3) {
+    // ---------------- producers: warp 0 K, warp 3 V ----------------
+    // (One warp for both took 2500 cycles a tile, 60 of them per box, and was what bounded the kernel.)
+    const bool is_v = warp == 3;
+    const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
+    const float* scale_src = is_v ? p.v_scale : p.k_scale;
+    if (lane == 0) ptx::prefetch_tmap(tm);
+    const int nb_shift = 31 - __clz(nb), j = lane & (nb - 1);  // nb is a power of two; this lane's block of a tile
+    const int tiles_per_block = rows == kTcTile ? p.block_size / kTcTile : 1;
     uint32_t it = 0;
     bool ok = true;
     // One code tile into the ring: lane j holds the id of the tile's block j.
-    auto load = [&](uint32_t n, const CUtensorMap* tm, int live, int x, int row, int blk) {
+    auto load = [&](uint32_t n, int live, int x, int row, int blk) {
       const uint32_t sl = slot_of(n);
       ok = ok && warp_wait(&empty_bar[sl], round_of(n) ^ 1, p.wait_ns);
       if (!ok || p.drop_loads) return;
@@ -531,15 +574,18 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (lane < live)
         q8::tma_load_3d(base_u32 + sl * L::kSlot + lane * rows * 128, tm, &full_bar[sl], x, row, blk);
     };
+    // V(t) follows K(t + 1) in the ring, so it is loaded once it is known whether there is one.
     int v_live = 0, v_x = 0, v_row = 0, v_blk = 0;
-    while (ok && w.next(p, s)) {
+    while (ok && next_share()) {
       const int pair = s.h / splits;
       const int32_t* bt = p.block_tables + (size_t)s.b * p.max_blocks;
       const int blk_end = (s.tok1 + p.block_size - 1) / p.block_size;
       constexpr int W = 4;  // ids of 128 blocks at a time, one per lane and register
       int win = -W * 32, id[W];
+      // the first block of the tile, and the tile's number in it where a block holds several
+      int first = s.tok0 / kTcTile * nb / tiles_per_block, sub = s.tok0 / kTcTile % tiles_per_block;
       for (int t0 = s.tok0; ok && t0 < s.tok1; t0 += kTcTile) {
-        const int first = t0 / p.block_size;
+        if (is_v && it > 0) load(v_at(it - 1), v_live, v_x, v_row, v_blk);  // before this tile's ids are waited for
         if (first + nb > win + W * 32) {
           win = first;
 #pragma unroll
@@ -549,43 +595,42 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           }
         }
         const int live = min(nb, blk_end - first);
-        const int rel = first + lane % nb - win;
+        const int rel = first + j - win;
         int blk = -1;
 #pragma unroll
         for (int r = 0; r < W; ++r) {
           const int v = __shfl_sync(0xffffffffu, id[r], rel & 31);
           blk = (rel >> 5) == r ? v : blk;
         }
-        load(k_at(it), &tm_k, live, pair * 128, t0 % p.block_size, blk);
+        if (!is_v) load(k_at(it), live, pair * 128, sub * kTcTile, blk);
         if (ok && !p.drop_loads) {
-          // scales [K, V][HP][nb]: this lane's block, K / V and heads by turns
-          const uint32_t scales = base_u32 + L::kScaleOff + (it % kScaleRing) * L::kScale;
-          const int j = lane % nb;
-          for (int i = lane / nb; i < 2 * HP; i += 32 / nb) {
-            const int kv = i & 1, hp = i >> 1, head = pair * HP + hp;
+          // scales [K, V][HP][nb]: this lane's block, heads by turns
+          const uint32_t scales = base_u32 + L::kScaleOff + (it % kScaleRing) * L::kScale + (is_v ? HP * nb * 4 : 0);
+          for (int hp = lane >> nb_shift; hp < HP; hp += 32 >> nb_shift) {
+            const int head = pair * HP + hp;
             const bool in = j < live && blk >= 0 && blk < p.num_blocks && head < Hkv;
-            const float* src = kv ? p.v_scale : p.k_scale;
-            q8::copy4_async(scales + ((kv * HP + hp) * nb + j) * 4, in ? src + (size_t)blk * Hkv + head : src, in);
+            q8::copy4_async(scales + (hp * nb + j) * 4, in ? scale_src + (size_t)blk * Hkv + head : scale_src, in);
           }
           q8::arrive_after_copies(&sc_full[it % kScaleRing]);
         }
-        if (it > 0) load(v_at(it - 1), &tm_v, v_live, v_x, v_row, v_blk);
         v_live = live;
         v_x = pair * 128;
-        v_row = t0 % p.block_size;
+        v_row = sub * kTcTile;
         v_blk = blk;
         ++it;
+        if (++sub == tiles_per_block) {
+          sub = 0;
+          first += nb;
+        }
       }
     }
-    uint32_t total = 0;
-    if (it > 0) {
-      total = v_at(it - 1);  // no K after the last tile: its place stays empty
-      load(total - 1, &tm_v, v_live, v_x, v_row, v_blk);
-    }
+    // The last V's place is the one that no further K takes.
+    if (is_v && it > 0) load(v_at(it - 1) - 1, v_live, v_x, v_row, v_blk);
     if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
     // No copy is in flight when the CTA ends, whatever became of the others.
+    const uint32_t total = 2 * it;
     for (uint32_t n = total > SL ? total - SL : 0; n < total && ok && !p.drop_loads; ++n)
-      ok = warp_wait(&full_bar[slot_of(n)], round_of(n), p.wait_ns);
+      if ((n == total - 1 || (n > 0 && n % 2 == 0)) == is_v) ok = warp_wait(&full_bar[slot_of(n)], round_of(n), p.wait_ns);
   } else if (warp == 1) {
     // ---------------- matrix issue: S^T of a tile, then P.V of the one before ----------------
     constexpr uint32_t idesc_s = umma::idesc_e4m3(128, L::NS, false);
@@ -615,7 +660,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       __syncwarp();
       due = false;
     };
-    while (ok && w.next(p, s)) {
+    while (ok && next_share()) {
       if (s.tok0 == s.tok1) continue;
       const uint32_t qb = share % QB;
       for (int t0 = s.tok0; ok && t0 < s.tok1; t0 += kTcTile) {
@@ -673,7 +718,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     constexpr int RPW = 32 / LPR;  // rows at a time
     uint32_t share = 0;
     bool ok = true;
-    while (ok && w.next(p, s)) {
+    while (ok && next_share()) {
       if (s.tok0 == s.tok1) continue;
       const uint32_t qb = share % QB;
       const int pair = s.h / splits, g0 = (s.h % splits) * GP;
@@ -735,25 +780,30 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         dead = true;
       }
     };
+    // The first query head of a share that this thread's rows of O^T belong to; Hq or more: none.
+    auto head_of = [&](const Share& x) -> int {
+      const int kvh = x.h / splits * HP + my_hp;
+      return kvh < Hkv ? kvh * G + x.h % splits * GP : p.n_heads;
+    };
+    auto heads_of = [&](const Share& x) { return min(GP, G - x.h % splits * GP); };  // per KV head
     // The next share with tokens; the rows of those without are zeros.
-    auto next_share = [&]() -> bool {
-      while (w.next(p, s)) {
+    auto next_live = [&]() -> bool {
+      while (next_share()) {
         if (s.ctx > 0) return true;
-        const int head = s.h / splits * HP + my_hp, g0 = (s.h % splits) * GP;
-        T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + (size_t)head * G + g0) * D + dim;
-        for (int h = 0; head < Hkv && h < min(GP, G - g0); ++h) out[(size_t)h * D] = DT<T>::from_f(0.f);
+        const int head0 = head_of(s);
+        T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + head0) * D + dim;
+        for (int h = 0; head0 < p.n_heads && h < heads_of(s); ++h) out[(size_t)h * D] = DT<T>::from_f(0.f);
       }
       return false;
     };
-    bool more = next_share();
+    // A piece has at most two shares of cut units, its first and its last.  Arriving at their units'
+    // counters takes round trips to memory, so it is left to the piece's end.
+    int n_cut = 0;
+    bool more = next_live();
     while (more) {
       const Share cur = s;
-      more = next_share();  // before this one is worked on, to know this CTA's last tile
-      const int pair = cur.h / splits, g0 = (cur.h % splits) * GP;
-      const int nh = min(GP, G - g0);  // query heads per KV head in this unit
-      T* out = reinterpret_cast<T*>(p.out) + (size_t)cur.b * p.n_heads * D;
-      const int head0 = (pair * HP + my_hp) * G + g0;  // this thread's first output head
-      const bool mine = pair * HP + my_hp < Hkv;
+      more = next_live();  // before this one is worked on, to know this CTA's last tile
+      const int nh = heads_of(cur);
       const uint32_t qb = share % QB;
       if (tid < HG) {  // heads beyond the group never ask for new references
         const float lim = tid % GP < nh ? -INFINITY : INFINITY;
@@ -916,70 +966,93 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (lane == 0) ptx::mbar_arrive(o_empty);
       ++share;
       ptx::named_barrier_sync(1, 128);
-      const int r0 = my_hp * GP;
-      float* part = cur.n_parts == 1 ? nullptr : part_slot(p, blockIdx.x, (int)blockIdx.x == cur.first_cta);
-#pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        if (h >= nh || !mine) continue;
-        const float2 ref = *reinterpret_cast<const float2*>(&ref_s[r0 + h].z);
-        const float A = (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * (ref.x == -INFINITY ? 0.f : ptx::ex2(ref.x - ref.y));
-        float Ls = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) Ls += red_s[k * 16 + r0 + h];
-        if (!part) {
-          out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(A / Ls);
-        } else {
-          __stcg(part + (r0 + h) * D + dim, A);
-          if (dim == 0) __stcg(reinterpret_cast<float2*>(part + HG * D + (r0 + h) * 2), make_float2(ref.y, Ls));
-        }
+      // Per head: what brings O^T from M to R, and the sum of weights; a whole unit's output is their quotient.
+      float* part = cur.n_parts == 1 ? nullptr : part_slot(p, blockIdx.x, cur.piece == cur.first_piece);
+      if (tid < HG) {
+        const float2 ref = *reinterpret_cast<const float2*>(&ref_s[tid].z);
+        const float sum = (red_s[tid] + red_s[16 + tid]) + (red_s[32 + tid] + red_s[48 + tid]);
+        const float f = ref.x == -INFINITY ? 0.f : ptx::ex2(ref.x - ref.y);
+        c_s[tid].x = part ? f : f / sum;
+        if (part) __stcg(reinterpret_cast<float2*>(part + HG * D + tid * 2), make_float2(ref.y, sum));
       }
+      ptx::named_barrier_sync(1, 128);
+      const int r0 = my_hp * GP, head0 = head_of(cur);
       if (part) {
-        auto sync = [] { ptx::named_barrier_sync(1, 128); };
-        if (last_to_arrive(p, cur, cur.b * units + cur.h, flag, tid, sync)) {
-          // All parts' (R, sum) at once: 8 threads a row; then the rows' weighted sums.  The weight
-          // buffers are free (their products are done): they take a factor per part and row.
-          float* f = reinterpret_cast<float*>(base + L::kPOff);
-          constexpr int kAtOnce = 2 * L::kP / 4 / HG;
-          float acc[GP];
-          const int row = tid >> 3;
-          const bool has = row < HG && row % GP < nh && pair * HP + row / GP < Hkv;
-          float M = -INFINITY, Ls = 0.f;
-          for (int c = tid & 7; has && c < cur.n_parts; c += 8)
-            M = fmaxf(M, __ldcg(part_slot(p, cur.first_cta + c, c == 0) + HG * D + row * 2));
 #pragma unroll
-          for (int d = 1; d < 8; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        for (int h = 0; h < GP; ++h)
+          __stcg(part + (r0 + h) * D + dim, (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * c_s[r0 + h].x);
+        if (tid == 0) cut_s[n_cut & 1] = cur;
+        ++n_cut;
+      } else if (head0 < p.n_heads) {
+        T* out = reinterpret_cast<T*>(p.out) + ((size_t)cur.b * p.n_heads + head0) * D + dim;
 #pragma unroll
-          for (int h = 0; h < GP; ++h) acc[h] = 0.f;
-          for (int c0 = 0; c0 < cur.n_parts; c0 += kAtOnce) {
-            const int c1 = min(cur.n_parts, c0 + kAtOnce);
-            for (int c = c0 + (tid & 7); has && c < c1; c += 8) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_slot(p, cur.first_cta + c, c == 0) + HG * D + row * 2));
-              const float e = exp2f(ml.x - M);
-              f[(c - c0) * HG + row] = e;
-              Ls = fmaf(ml.y, e, Ls);
-            }
-            sync();
-            if (mine) {
-#pragma unroll 4
-              for (int c = c0; c < c1; ++c) {
-                const float* src = part_slot(p, cur.first_cta + c, c == 0) + r0 * D + dim;
+        for (int h = 0; h < GP; ++h)
+          if (h < nh) out[(size_t)h * D] = DT<T>::from_f((fmaf(o2[h], kLowPart, o1[h]) + o[h]) * c_s[r0 + h].x);
+      }
+    }
+
+    // ---------------- cut units: arrive, and where this is the last to, add the parts up ----------------
+    for (int i = 0; i < n_cut; ++i) {
+      auto sync = [] { ptx::named_barrier_sync(1, 128); };
+      sync();  // cut_s is written
+      const Share cur = cut_s[i];
+      if (!last_to_arrive(p, cur, cur.b * units + cur.h, flag, tid, sync)) continue;
+      const int r0 = my_hp * GP, head0 = head_of(cur), nh = heads_of(cur), n_parts = cur.n_parts;
+      // First the factor of every part and row, 8 threads a row, then the rows' weighted sums.  The
+      // weight buffers are free (their products are done): they take the factors.
+      const float* parts = part_slot(p, cur.first_piece * team + mate, false);
+      auto at_part = [&](int c) { return c == 0 ? kSlotFloats : c * team * 2 * kSlotFloats; };  // as part_slot places them
+      float* f = reinterpret_cast<float*>(base + L::kPOff);
+      constexpr int kAtOnce = 2 * L::kP / 4 / HG;
+      const int row = tid >> 3;
+      const bool has = row < HG;
+      const float* ml_row = parts + HG * D + row * 2;
+      float M = -INFINITY, Ls = 0.f;
+      float2 ml = make_float2(-INFINITY, 0.f);  // of one of the first 8 parts, read once
+      if (has && (tid & 7) < n_parts) ml = __ldcg(reinterpret_cast<const float2*>(ml_row + at_part(tid & 7)));
+      M = ml.x;
+      for (int c = (tid & 7) + 8; has && c < n_parts; c += 8) M = fmaxf(M, __ldcg(ml_row + at_part(c)));
 #pragma unroll
-                for (int h = 0; h < GP; ++h)
-                  if (h < nh) acc[h] = fmaf(__ldcg(src + h * D), f[(c - c0) * HG + r0 + h], acc[h]);
-              }
-            }
-            sync();
+      for (int d = 1; d < 8; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+      float acc[GP];
+#pragma unroll
+      for (int h = 0; h < GP; ++h) acc[h] = 0.f;
+      for (int c0 = 0; c0 < n_parts; c0 += kAtOnce) {
+        const int n = min(n_parts - c0, kAtOnce);
+        for (int c = tid & 7; has && c < n; c += 8) {
+          const float2 x = c0 + c < 8 ? ml : __ldcg(reinterpret_cast<const float2*>(ml_row + at_part(c0 + c)));
+          const float e = exp2f(x.x - M);
+          f[c * HG + row] = e;
+          Ls = fmaf(x.y, e, Ls);
+        }
+        sync();
+        constexpr int U = GP >= 8 ? 4 : 8;  // parts whose sums are in flight together
+        const float* src = parts + r0 * D + dim;
+        for (int c = 0; c < n; c += U) {
+          float v[U][GP];
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            const float* at = src + at_part(c0 + min(c + k, n - 1));
+#pragma unroll
+            for (int h = 0; h < GP; ++h) v[k][h] = __ldcg(at + h * D);
           }
 #pragma unroll
-          for (int d = 1; d < 8; d <<= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, d);
-          if (has && (tid & 7) == 0) red_s[row] = Ls;
-          sync();
+          for (int k = 0; k < U; ++k)
 #pragma unroll
-          for (int h = 0; h < GP; ++h)
-            if (mine && h < nh) out[(size_t)(head0 + h) * D + dim] = DT<T>::from_f(acc[h] / red_s[r0 + h]);
+            for (int h = 0; h < GP; ++h)
+              acc[h] = fmaf(v[k][h], c + k < n ? f[(c + k) * HG + r0 + h] : 0.f, acc[h]);
         }
+        sync();
       }
-      ptx::named_barrier_sync(1, 128);  // red_s and ref_s have been read
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, d);
+      if (has && (tid & 7) == 0) red_s[row] = Ls;
+      sync();
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)cur.b * p.n_heads + head0) * D + dim;
+#pragma unroll
+      for (int h = 0; h < GP; ++h)
+        if (head0 < p.n_heads && h < nh) out[(size_t)h * D] = DT<T>::from_f(acc[h] / red_s[r0 + h]);
+      sync();  // red_s and the factors may be written again
     }
   }
   umma::fence_before_sync();
@@ -993,8 +1066,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 template <typename T>
 int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
   const long long most = (long long)p.batch * p.n_kv_heads * (tiles_of(p.max_ctx_tokens, kSimtTile) + kUnitTiles);
-  const long long pieces = (most + kMinPiece - 1) / kMinPiece;
-  const int grid = (int)(pieces < kMaxCtas ? pieces : kMaxCtas);
+  const int grid = (int)(most < kSimtCtas ? most : kSimtCtas);
   switch (head_dim) {
     case 32: TVK_CHECK_CUDA(tvk::launch_pdl(paged_decode_q8_simt_kernel<T, 32>, grid, 128, 0, stream, p)); break;
     case 64: TVK_CHECK_CUDA(tvk::launch_pdl(paged_decode_q8_simt_kernel<T, 64>, grid, 128, 0, stream, p)); break;
@@ -1038,10 +1110,15 @@ int launch_tc(const Q8Params& p, cudaStream_t stream) {
     if (dev < 64) attr_set.fetch_or(1ull << dev);
   }
   const int units = (p.n_kv_heads + L::HP - 1) / L::HP * ((p.group + GP - 1) / GP);
-  const long long most = (long long)p.batch * units * (tiles_of(p.max_ctx_tokens, kTcTile) + kUnitTiles);
-  const long long pieces = (most + kMinPiece - 1) / kMinPiece;
-  const int grid = (int)(pieces < kTcCtas ? pieces : kTcCtas);
-  TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, kTcThreads, L::kBytes, stream, p, tm[0], tm[1]));
+  // Teams of up to 8 CTAs on neighbouring units of the same tokens: what they read lies side by side in
+  // the pool, and they read it at about the same time.
+  int team = units < 8 ? units : 8;
+  while (units % team) --team;
+  const long long most = (long long)p.batch * (units / team) * (tiles_of(p.max_ctx_tokens, kTcTile) + kUnitTiles);
+  const int pieces = (int)(most < kTcCtas / team ? most : kTcCtas / team);
+  Q8Params q = p;
+  q.team = team;
+  TVK_CHECK_CUDA(tvk::launch_pdl(kern, pieces * team, kTcThreads, L::kBytes, stream, q, tm[0], tm[1]));
   TVK_CHECK_LAUNCH("paged_decode_q8_tc");
   return TVK_OK;
 }
@@ -1062,7 +1139,7 @@ int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
 
 extern "C" size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads) {
   const size_t units = batch > 0 && n_kv_heads > 0 ? (size_t)batch * n_kv_heads * kMaxParts : 0;
-  return tvk::kWorkspaceHeader + (size_t)2 * kMaxCtas * kSlotFloats * sizeof(float) + units * sizeof(int);
+  return tvk::kWorkspaceHeader + (size_t)2 * kMaxPieces * kSlotFloats * sizeof(float) + units * sizeof(int);
 }
 
 extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache, const void* v_cache,
@@ -1109,7 +1186,7 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
   p.v_scale = v_scale;
   p.status = (int*)workspace;
   p.part = (float*)((uint8_t*)workspace + tvk::kWorkspaceHeader);
-  p.counters = (int*)(p.part + (size_t)2 * kMaxCtas * kSlotFloats);
+  p.counters = (int*)(p.part + (size_t)2 * kMaxPieces * kSlotFloats);
   p.batch = batch;
   p.n_heads = n_heads;
   p.n_kv_heads = n_kv_heads;
