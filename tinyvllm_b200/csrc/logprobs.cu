@@ -10,13 +10,16 @@
 // Each thread keeps (m, S, T) in fp32 for the logits it reads, 16 bytes at a
 // time, and moves m only when a vector exceeds it.
 //
-// The K best: after the first tile (512 threads x 4 vectors) the CTA picks a
-// threshold that at least K threads' maxima reach, so at least K logits of
-// the row do; a logit below it cannot be among the K best.  What reaches it is
-// pushed as a 64-bit key (ordered value, inverted index) to shared memory, and
-// the K best of those few hundred keys are found by bisection over the keys.
+// The K best: from the maxima of 32 groups of threads over the first tile (512
+// threads x 4 vectors) each CTA takes the K-th largest as a threshold, which K
+// logits at least reach; one below it is not among the K best.  What reaches it is
+// pushed as a 64-bit key (ordered value, inverted index) to shared memory, and the
+// K best of those few hundred keys are found by bisection and ranking.
 // Rows that keep pushing (sorted or constant logits) run into the buffer's
 // limit, are cut back to their K best and go on with an exact threshold.
+//
+// With few rows a cluster of CTAs shares each: the CTAs' sums and K best are put
+// together by the first over distributed shared memory.
 #include <math.h>
 
 #include "tvk_common.cuh"
@@ -63,46 +66,97 @@ template <> __device__ __forceinline__ float vec_max<__nv_bfloat16>(const uint4&
   return __bfloat162float(__hmax_nan(c.x, c.y));
 }
 
-// Running sums of one thread: s = sum exp(x - m), t = sum exp(x - m) (x - m).
-// x - m is formed before the scaling to base 2, so rows that hold nothing but
-// the type's lowest value (masks) neither overflow nor cancel.
-struct Sums {
-  float m, s, t;
+// Two fp32 values in one register pair, for the packed fp32 instructions.
+struct F2 {
+  uint64_t v;
 };
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Elements 2 i and 2 i + 1 of a 16-byte vector.
+template <typename T> __device__ __forceinline__ F2 pair_of(const uint4& u, int i);
+template <> __device__ __forceinline__ F2 pair_of<float>(const uint4& u, int i) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+  return pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
+template <> __device__ __forceinline__ F2 pair_of<__half>(const uint4& u, int i) {
+  const float2 f = __half22float2(reinterpret_cast<const __half2*>(&u)[i]);
+  return pack(f.x, f.y);
+}
+template <> __device__ __forceinline__ F2 pair_of<__nv_bfloat16>(const uint4& u, int i) {
+  const uint32_t w = reinterpret_cast<const uint32_t*>(&u)[i];
+  return pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Running sums of one thread, even and odd elements apart: s = sum exp(x - m),
+// t = sum exp(x - m) (x - m).  x - m is formed before the scaling to base 2, so rows
+// that hold nothing but the type's lowest value (masks) neither overflow nor cancel.
+struct Sums {
+  float m;
+  F2 s, t;
+};
+
+// c (t + d s) for a move of the reference by d, c = exp(d); 0 where c is (d s may overflow there).
+__device__ __forceinline__ float moved(float c, float d, float s, float t) { return c == 0.f ? 0.f : c * fmaf(d, s, t); }
 
 // New maximum: m > a.m, or NaN (then everything becomes NaN, as it should).
 __device__ __forceinline__ void raise_max(Sums& a, float m) {
   if (a.m == -INFINITY) {  // nothing but -inf so far
-    a.s = a.t = m != m ? m : 0.f;
+    const float z = m != m ? m : 0.f;
+    a.s = a.t = pack(z, z);
   } else {
     const float d = a.m - m, c = ptx::ex2(d * kLog2e);
-    a.t = c == 0.f ? 0.f : c * fmaf(d, a.s, a.t);  // d * s may overflow where c is 0
-    a.s *= c;
+    const float2 s = unpack(a.s), t = unpack(a.t);
+    a.t = pack(moved(c, d, s.x, t.x), moved(c, d, s.y, t.y));
+    a.s = mul2(a.s, pack(c, c));
   }
   a.m = m;
 }
 
-__device__ __forceinline__ void add(Sums& a, float x, float m) {
+__device__ __forceinline__ void add_pair(Sums& a, F2 x, F2 minus_m) {
   // exp(-200) is 0 here: -inf adds 0 * -200 to t, not 0 * -inf; NaN stays
-  const float d = max_nan(x - m, -200.f);
-  const float e = ptx::ex2(d * kLog2e);
-  a.s += e;
-  a.t = fmaf(e, d, a.t);
+  float2 d = unpack(add2(x, minus_m));
+  d.x = max_nan(d.x, -200.f);
+  d.y = max_nan(d.y, -200.f);
+  const F2 dd = pack(d.x, d.y);
+  const float2 u = unpack(mul2(dd, pack(kLog2e, kLog2e)));
+  const F2 e = pack(ptx::ex2(u.x), ptx::ex2(u.y));
+  a.s = add2(a.s, e);
+  a.t = fma2(e, dd, a.t);
 }
 
-__device__ __forceinline__ Sums merge(const Sums& a, const Sums& b) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  r.s = r.t = 0.f;
-  const Sums* p[2] = {&a, &b};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (p[i]->m == -INFINITY && p[i]->s == 0.f) continue;  // nothing but -inf seen
-    const float d = p[i]->m - r.m, c = ptx::ex2(d * kLog2e);
-    r.s += p[i]->s * c;
-    r.t += c == 0.f ? 0.f : c * fmaf(d, p[i]->s, p[i]->t);
-  }
-  return r;
+// Sums relative to one maximum.
+struct RowSums {
+  float m, s, t;
+};
+// a's sums with the reference moved to m >= a.m.
+__device__ __forceinline__ RowSums at_max(const RowSums& a, float m) {
+  if (a.m == -INFINITY && a.s == 0.f) return RowSums{m, 0.f, 0.f};  // nothing but -inf seen
+  const float d = a.m - m, c = ptx::ex2(d * kLog2e);
+  return RowSums{m, a.s * c, moved(c, d, a.s, a.t)};
 }
 
 struct LpParams {
@@ -118,10 +172,12 @@ struct LpParams {
 
 struct LpShared {
   unsigned long long keys[kLpBuf];
-  unsigned long long best[kLpMaxK];
-  Sums part[kLpThreads / 32];
-  Sums row;
-  int count;
+  unsigned long long best[kLpMaxK];  // this CTA's K best, in order
+  RowSums sums;                      // and its part of the row's sums
+  RowSums all_sums[8];
+  float part[kLpThreads / 32][2];
+  uint32_t group_max[32];
+  int count, n_best;
   int wsum[kLpThreads / 32];
 };
 
@@ -189,28 +245,102 @@ __device__ __forceinline__ unsigned long long key_of(float x, int idx) {
   return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - (uint32_t)idx);
 }
 
-// One CTA per row.
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared variable in another CTA of the cluster.
+template <typename P>
+__device__ __forceinline__ const P* of_cta(const P* x, uint32_t rank) {
+  uint64_t r;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(x)), "r"(rank));
+  return reinterpret_cast<const P*>(r);
+}
+
+// Sum and maximum over the CTA, the same in every thread.
+__device__ __forceinline__ float block_max(LpShared& sh, float x) {
+  float w;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(w) : "f"(x));
+  if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5][0] = w;
+  __syncthreads();
+  float m = sh.part[0][0];
+#pragma unroll
+  for (int i = 1; i < kLpThreads / 32; ++i) m = fmaxf(m, sh.part[i][0]);
+  __syncthreads();
+  return m;
+}
+
+// The K best keys of the buffer, in order, into sh.best; fewer if there are no more.
+__device__ void select_best(LpShared& sh, int K, unsigned long long* scratch_kth) {
+  __syncthreads();
+  int n = sh.count;
+  const int tid = threadIdx.x;
+  if (n > 64) {
+    bool few = false;
+    if (n <= kLpThreads) {
+      // one key a thread: bisection over the values alone, until at most 64 keys are left
+      const unsigned long long k = tid < n ? sh.keys[tid] : 0ull;
+      const uint32_t o = (uint32_t)(k >> 32);
+      uint32_t lo = 0u, hi = 0xffffffffu;  // count(o >= lo) >= K; the same below hi need not hold
+      while (!few && hi - lo > 1u) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        const int c = __syncthreads_count(tid < n && o >= mid);
+        if (c >= K) {
+          lo = mid;
+          few = c <= 64;
+        } else {
+          hi = mid;
+        }
+      }
+      if (few) {
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        if (tid < n && o >= lo) sh.keys[atomicAdd(&sh.count, 1)] = k;
+        __syncthreads();
+        n = sh.count;
+      }
+    }
+    if (!few) n = keep_best(sh, K, 0, 0, scratch_kth);
+  }
+  if (tid < n) {
+    const unsigned long long k = sh.keys[tid];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.keys[j] > k;
+    if (rank < K) sh.best[rank] = k;
+  }
+  if (tid == 0) sh.n_best = n < K ? n : K;
+}
+
+// One cluster (of one CTA or more) per row.
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpParams p) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
   constexpr int N = 16 / sizeof(T);
   __shared__ LpShared sh;
-  const int K = p.top_k, V = p.vocab, tid = threadIdx.x;
-  const long long row = blockIdx.x;
+  const int K = p.top_k, V = p.vocab, tid = threadIdx.x, lane = tid & 31;
+  const uint32_t ctas = cluster_size(), rank = blockIdx.x % ctas;
+  const long long row = blockIdx.x / ctas;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.row_stride;
   float x_tok = 0.f;
   bool inside = false;  // a token outside the vocabulary has probability 0
   if (tid == 0) {
     sh.count = 0;
-    const int tok = p.tokens[row];
-    inside = tok >= 0 && tok < V;
-    if (inside) x_tok = DT<T>::to_f(x[tok]);
+    if (rank == 0) {
+      const int tok = p.tokens[row];
+      inside = tok >= 0 && tok < V;
+      if (inside) x_tok = DT<T>::to_f(x[tok]);
+    }
   }
   // Elements before the first 16-byte boundary and after the last whole vector go one to a thread.
   const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int nvec = (V - head) / N, tail0 = head + nvec * N;
+  const int all_vec = (V - head) / N, tail0 = head + all_vec * N;
   const T* xv = x + head;
-  Sums a{-INFINITY, 0.f, 0.f};
+  const int v0 = (int)((long long)all_vec * rank / ctas), v1 = (int)((long long)all_vec * (rank + 1) / ctas);
+  Sums a{-INFINITY, pack(0.f, 0.f), pack(0.f, 0.f)};
   unsigned long long tau_key = 0ull;  // only keys above it are candidates
   float tau = -INFINITY;              // only values not below it are
   __syncthreads();
@@ -223,63 +353,60 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     return at >= kLpBuf / 2;
   };
 
-  {
+  if (rank == 0) {
     const int single = tid < head ? tid : (tid < head + V - tail0 ? tail0 + tid - head : -1);
     if (single >= 0) {
       const float f = DT<T>::to_f(x[single]);
       raise_max(a, f);
-      add(a, f, a.m == -INFINITY ? 0.f : a.m);
+      const float ref = a.m == -INFINITY ? 0.f : a.m;
+      add_pair(a, pack(f, -INFINITY), pack(-ref, -ref));
       if (K > 0) push(f, single);
     }
   }
 
-  for (int base = 0; base < nvec; base += kLpThreads * kLpUnroll) {
+  for (int base = v0; base < v1; base += kLpThreads * kLpUnroll) {
     uint4 u[kLpUnroll];
     float vm[kLpUnroll];
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
       const int i = base + k * kLpThreads + tid;
-      if (i < nvec) u[k] = __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
+      if (i < v1) u[k] = __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
     }
     float tm = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
-      if (base + k * kLpThreads + tid < nvec) {
+      if (base + k * kLpThreads + tid < v1) {
         vm[k] = vec_max<T>(u[k]);
         tm = max_nan(tm, vm[k]);
         if (!(vm[k] <= a.m)) raise_max(a, vm[k]);
         const float ref = a.m == -INFINITY ? 0.f : a.m;
-        const T* h = reinterpret_cast<const T*>(&u[k]);
+        const F2 minus_m = pack(-ref, -ref);
 #pragma unroll
-        for (int e = 0; e < N; ++e) add(a, DT<T>::to_f(h[e]), ref);
+        for (int e = 0; e < N / 2; ++e) add_pair(a, pair_of<T>(u[k], e), minus_m);
       }
     }
     if (K == 0) continue;
-    if (base == 0) {
-      // A value that between K and 2K threads' maxima reach (by bisection; fewer
-      // steps than the exact K-th needs): K logits at least are not below it.
-      const bool has = tid < nvec;
-      const uint32_t o = has ? order_of(tm) : 0u;
-      if (__syncthreads_count(has) >= K) {
-        uint32_t lo = 0u, hi = 0xffffffffu;
-        while (hi - lo > 1u) {
-          const uint32_t mid = lo + ((hi - lo) >> 1);
-          const int c = __syncthreads_count(has && o >= mid);
-          if (c >= K) {
-            lo = mid;
-            if (c <= 2 * K) break;
-          } else {
-            hi = mid;
-          }
-        }
-        if (lo) tau = value_of(lo);
+    if (base == v0) {
+      // The K-th largest of the maxima of 32 groups of 16 threads: K logits at least are not below it.
+      const uint32_t o = tid < v1 - v0 ? order_of(tm) : 0u;
+      const uint32_t top = __reduce_max_sync(lane < 16 ? 0x0000ffffu : 0xffff0000u, o);
+      if ((lane & 15) == 0) sh.group_max[tid >> 4] = top;
+      __syncthreads();
+      const uint32_t mine = sh.group_max[lane];
+      int above = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+        above += other > mine || (other == mine && j < lane);
       }
+      const uint32_t at_k = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, above == K - 1)) - 1);
+      if (at_k) tau = value_of(at_k);  // 0: fewer than K groups have elements
     }
     bool full = false;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
       const int i = base + k * kLpThreads + tid;
-      if (i < nvec && !(vm[k] < tau)) {
+      if (i < v1 && !(vm[k] < tau)) {
         const T* h = reinterpret_cast<const T*>(&u[k]);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -294,11 +421,11 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     } else {
       // Keys of this tile were lost: take the tile out and push it again, one
       // element a thread at a time, cutting back whenever the next step might overflow.
-      keep_best(sh, K, head + base * N, head + min(base + kLpThreads * kLpUnroll, nvec) * N, &tau_key);
+      keep_best(sh, K, head + base * N, head + min(base + kLpThreads * kLpUnroll, v1) * N, &tau_key);
       for (int k = 0; k < kLpUnroll; ++k) {
         const int i = base + k * kLpThreads + tid;
         for (int e = 0; e < N; ++e) {
-          if (i < nvec) push(DT<T>::to_f(xv[(size_t)i * N + e]), head + i * N + e);
+          if (i < v1) push(DT<T>::to_f(xv[(size_t)i * N + e]), head + i * N + e);
           __syncthreads();
           const bool cut = sh.count > kLpBuf - kLpThreads;
           __syncthreads();
@@ -310,48 +437,92 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     if (tau_key) tau = value_of((uint32_t)(tau_key >> 32));
   }
 
-  // sums of the row
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-    a = merge(a, b);
-  }
-  if ((tid & 31) == 0) sh.part[tid >> 5] = a;
-  __syncthreads();
-  if (tid < 32) {
-    a = tid < kLpThreads / 32 ? sh.part[tid] : Sums{-INFINITY, 0.f, 0.f};
+  // This CTA's sums: the maximum first, then every thread's sums relative to it.
+  {
+    const float m = block_max(sh, a.m);
+    const float2 s2 = unpack(a.s), t2 = unpack(a.t);
+    const RowSums mine = at_max(RowSums{a.m, s2.x + s2.y, t2.x + t2.y}, m);
+    float s = mine.s, t = mine.t;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      Sums b;
-      b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-      b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-      a = merge(a, b);
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
     }
-    if (tid == 0) sh.row = a;
+    if (lane == 0) {
+      sh.part[tid >> 5][0] = s;
+      sh.part[tid >> 5][1] = t;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      s = t = 0.f;
+#pragma unroll
+      for (int i = 0; i < kLpThreads / 32; ++i) {
+        s += sh.part[i][0];
+        t += sh.part[i][1];
+      }
+      sh.sums = RowSums{m, s, t};
+    }
   }
-  __syncthreads();
-  const Sums r = sh.row;
-  const float log_s = logf(r.s);
-  // x - lse; a row of nothing but -inf gives NaN for every token, as the formula does
-  auto logprob = [&](float f) -> float { return (f - r.m) - log_s; };
-  if (tid == 0) {
-    p.logprobs[row] = inside ? logprob(x_tok) : -INFINITY;
-    p.entropy[row] = log_s - r.t / r.s;
-  }
-  if (K > 0) {
-    const int n = keep_best(sh, K, 0, 0, &tau_key);
-    if (tid < n) {
+  if (K > 0) select_best(sh, K, &tau_key);
+  if (ctas > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+
+  if (rank == 0) {
+    // All CTAs' sums and K best to this one's shared memory, then the row's by every thread that writes
+    // something.  (A CTA's places behind its last key hold 0, which no key is.)
+    const int n_all = (int)ctas * K;
+    if (tid < (int)ctas) sh.all_sums[tid] = *of_cta(&sh.sums, tid);
+    if (tid < n_all) {
+      const uint32_t c = tid / K;
+      const int i = tid % K;
+      sh.keys[tid] = i < *of_cta(&sh.n_best, c) ? of_cta(sh.best, c)[i] : 0ull;
+    }
+    __syncthreads();
+    RowSums r = sh.all_sums[0];
+    for (uint32_t c = 1; c < ctas; ++c) {
+      const RowSums other = sh.all_sums[c];
+      const float m = fmaxf(r.m, other.m);
+      const RowSums x0 = at_max(r, m), x1 = at_max(other, m);
+      r = RowSums{m, x0.s + x1.s, x0.t + x1.t};
+    }
+    const float log_s = logf(r.s);
+    // x - lse; a row of nothing but -inf gives NaN for every token, as the formula does
+    auto logprob = [&](float f) -> float { return (f - r.m) - log_s; };
+    if (tid == 0) {
+      p.logprobs[row] = inside ? logprob(x_tok) : -INFINITY;
+      p.entropy[row] = log_s - r.t / r.s;
+    }
+    // The row's K best are those of all CTAs' K best that fewer than K others exceed.
+    if (tid < n_all && sh.keys[tid] != 0ull) {
       const unsigned long long k = sh.keys[tid];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sh.keys[j] > k;
-      p.top_logprobs[row * K + rank] = logprob(value_of((uint32_t)(k >> 32)));
-      p.top_tokens[row * K + rank] = (int)(0xffffffffu - (uint32_t)k);
+      int place = 0;
+      for (int j = 0; j < n_all; ++j) place += sh.keys[j] > k;
+      if (place < K) {
+        p.top_logprobs[row * K + place] = logprob(value_of((uint32_t)(k >> 32)));
+        p.top_tokens[row * K + place] = (int)(0xffffffffu - (uint32_t)k);
+      }
     }
   }
+  if (ctas > 1) cluster_sync();  // no CTA ends while its shared memory is read
+}
+
+template <typename T>
+cudaError_t launch_logprobs(const LpParams& p, int rows, int ctas, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * ctas);
+  cfg.blockDim = kLpThreads;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = tvk::pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p);
 }
 
 }  // namespace
@@ -368,14 +539,17 @@ extern "C" int tvk_token_logprobs(const void* logits, const int32_t* tokens, flo
   TVK_CHECK_ARG(logits && tokens && logprobs && entropy && (top_k == 0 || (top_logprobs && top_tokens)),
                 "null pointer argument");
   TVK_CHECK_ARG((uintptr_t)logits % tvk::dtype_size(dtype) == 0, "logits must be aligned to their elements");
-  LpParams p{logits, tokens, logprobs, entropy, top_logprobs, top_tokens, row_stride, vocab, top_k};
+  const LpParams p{logits, tokens, logprobs, entropy, top_logprobs, top_tokens, row_stride, vocab, top_k};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  // CTAs per row: as many as keep all rows resident at once (two CTAs on each of 148
+  // SMs), but none with less than a tile of its own.
+  const long long vecs = (long long)vocab * (long long)tvk::dtype_size(dtype) / 16;
+  int ctas = 8;
+  while (ctas > 1 && ((long long)rows * ctas > 296 || vecs < (long long)ctas * kLpThreads)) ctas >>= 1;
   switch (dtype) {
-    case TVK_DTYPE_F16: TVK_CHECK_CUDA(tvk::launch_pdl(token_logprobs_kernel<__half>, rows, kLpThreads, 0, s, p)); break;
-    case TVK_DTYPE_BF16:
-      TVK_CHECK_CUDA(tvk::launch_pdl(token_logprobs_kernel<__nv_bfloat16>, rows, kLpThreads, 0, s, p));
-      break;
-    default: TVK_CHECK_CUDA(tvk::launch_pdl(token_logprobs_kernel<float>, rows, kLpThreads, 0, s, p)); break;
+    case TVK_DTYPE_F16: TVK_CHECK_CUDA(launch_logprobs<__half>(p, rows, ctas, s)); break;
+    case TVK_DTYPE_BF16: TVK_CHECK_CUDA(launch_logprobs<__nv_bfloat16>(p, rows, ctas, s)); break;
+    default: TVK_CHECK_CUDA(launch_logprobs<float>(p, rows, ctas, s)); break;
   }
   TVK_CHECK_LAUNCH("token_logprobs");
   return TVK_OK;
