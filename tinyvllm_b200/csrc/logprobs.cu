@@ -8,13 +8,15 @@
 //   top[r]     = the K largest logits, equal values in index order
 //
 // Each thread keeps (m, S, T) in fp32 for the logits it reads, 16 bytes at a
-// time, and moves m only when a vector exceeds it.
+// time; its m moves only when a vector exceeds it by more than 4 (moving at every new
+// maximum, some lane of a warp did so in most steps, which cost a third of the time).
 //
-// The K best: from the maxima of 32 groups of threads over the first tile (512
-// threads x 4 vectors) each CTA takes the K-th largest as a threshold, which K
+// The K best: from the maxima of 32 groups of threads over the first step (4
+// vectors a thread) each CTA takes the K-th largest as a threshold, which K
 // logits at least reach; one below it is not among the K best.  What reaches it is
-// pushed as a 64-bit key (ordered value, inverted index) to shared memory, and the
-// K best of those few hundred keys are found by bisection and ranking.
+// pushed as a 64-bit key (ordered value, inverted index) to shared memory; the same
+// with groups of keys raises the threshold once more after a few steps, and leaves little
+// more than the K best for ranking at the end.
 // Rows that keep pushing (sorted or constant logits) run into the buffer's
 // limit, are cut back to their K best and go on with an exact threshold.
 //
@@ -22,16 +24,19 @@
 // together by the first over distributed shared memory.
 #include <math.h>
 
+#include <type_traits>
+
 #include "tvk_common.cuh"
 
 namespace {
 
-constexpr int kLpThreads = 512;
 constexpr int kLpUnroll = 4;         // 16-byte loads in flight per thread
+constexpr int kLpSteps = 4;          // steps between two looks at the candidate buffer
+constexpr float kLpSlack = 4.f;      // a reference may lie this far below its thread's largest logit
 constexpr int kLpBuf = 2048;         // candidate keys kept in shared memory
 constexpr int kLpMaxK = 32;
-constexpr int kLpPerThread = kLpBuf / kLpThreads;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLpFloor = -30000.f;  // see add_vec
 
 // fp32 values as unsigned integers of the same order: -0 counts as +0, every
 // NaN as one value above +inf.
@@ -64,6 +69,39 @@ template <> __device__ __forceinline__ float vec_max<__nv_bfloat16>(const uint4&
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
   const __nv_bfloat162 c = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
   return __bfloat162float(__hmax_nan(c.x, c.y));
+}
+
+// Element e of a vector, without a register array.
+template <typename T> __device__ __forceinline__ T element(const uint4& u, int e) {
+  const uint32_t w = sizeof(T) == 4 ? (e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w)
+                                    : (e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w);
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w);
+  } else {
+    const uint16_t b = (uint16_t)(e & 1 ? w >> 16 : w);
+    return *reinterpret_cast<const T*>(&b);
+  }
+}
+
+// Bit e: element e is not below tau (NaN is not).  tau is -inf, NaN or an element's value, so the 16-bit types hold it.
+template <typename T> __device__ __forceinline__ uint32_t not_below(const uint4& u, float tau) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t bits = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= (uint32_t)!(__uint_as_float(w[i]) < tau) << i;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T t = DT<T>::from_f(tau);
+    T2 t2;
+    t2.x = t2.y = t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = ~__hlt2_mask(*reinterpret_cast<const T2*>(&w[i]), t2);
+      bits |= (m & 1u) << (2 * i) | (m >> 31) << (2 * i + 1);
+    }
+  }
+  return bits;
 }
 
 // Two fp32 values in one register pair, for the packed fp32 instructions.
@@ -111,24 +149,38 @@ template <> __device__ __forceinline__ F2 pair_of<__nv_bfloat16>(const uint4& u,
   return pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// The vector with every element raised to at least -30000 (16-bit types; NaN stays), and for fp32 itself.
+template <typename T> __device__ __forceinline__ uint4 floored(const uint4& u) {
+  uint4 r = u;
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T low = DT<T>::from_f(kLpFloor);
+    T2 low2;
+    low2.x = low2.y = low;
+    T2* h = reinterpret_cast<T2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low2);
+  }
+  return r;
+}
+
 // Running sums of one thread, even and odd elements apart: s = sum exp(x - m),
-// t = sum exp(x - m) (x - m).  x - m is formed before the scaling to base 2, so rows
-// that hold nothing but the type's lowest value (masks) neither overflow nor cancel.
+// t = sum exp(x - m) u, u = (x - m) / ln 2.
 struct Sums {
   float m;
   F2 s, t;
 };
 
-// c (t + d s) for a move of the reference by d, c = exp(d); 0 where c is (d s may overflow there).
+// c (t + d s) for a move of the reference by d, c = 2^d; 0 where c is (d s may overflow there).
 __device__ __forceinline__ float moved(float c, float d, float s, float t) { return c == 0.f ? 0.f : c * fmaf(d, s, t); }
 
-// New maximum: m > a.m, or NaN (then everything becomes NaN, as it should).
+// New reference: m > a.m, or NaN (then everything becomes NaN, as it should).
 __device__ __forceinline__ void raise_max(Sums& a, float m) {
   if (a.m == -INFINITY) {  // nothing but -inf so far
     const float z = m != m ? m : 0.f;
     a.s = a.t = pack(z, z);
   } else {
-    const float d = a.m - m, c = ptx::ex2(d * kLog2e);
+    const float d = (a.m - m) * kLog2e, c = ptx::ex2(d);
     const float2 s = unpack(a.s), t = unpack(a.t);
     a.t = pack(moved(c, d, s.x, t.x), moved(c, d, s.y, t.y));
     a.s = mul2(a.s, pack(c, c));
@@ -136,16 +188,39 @@ __device__ __forceinline__ void raise_max(Sums& a, float m) {
   a.m = m;
 }
 
-__device__ __forceinline__ void add_pair(Sums& a, F2 x, F2 minus_m) {
-  // exp(-200) is 0 here: -inf adds 0 * -200 to t, not 0 * -inf; NaN stays
-  float2 d = unpack(add2(x, minus_m));
-  d.x = max_nan(d.x, -200.f);
-  d.y = max_nan(d.y, -200.f);
-  const F2 dd = pack(d.x, d.y);
-  const float2 u = unpack(mul2(dd, pack(kLog2e, kLog2e)));
-  const F2 e = pack(ptx::ex2(u.x), ptx::ex2(u.y));
+// With any reference.  x - m is formed before the scaling to base 2, so rows that hold nothing
+// but the type's lowest value (masks) neither overflow nor cancel.
+__device__ __forceinline__ void add_pair(Sums& a, F2 x) {
+  const float ref = a.m == -INFINITY ? 0.f : a.m;
+  // 2^-300 is 0 here: -inf adds 0 * -300 to t, not 0 * -inf; NaN stays
+  const float2 d = unpack(add2(x, pack(-ref, -ref)));
+  const F2 u = pack(max_nan(d.x * kLog2e, -300.f), max_nan(d.y * kLog2e, -300.f));
+  const float2 v = unpack(u);
+  const F2 e = pack(ptx::ex2(v.x), ptx::ex2(v.y));
   a.s = add2(a.s, e);
-  a.t = fma2(e, dd, a.t);
+  a.t = fma2(e, u, a.t);
+}
+
+// A whole vector.  With an ordinary reference (almost always) 16-bit elements are floored two
+// at a time: what lies below -30000 weighs nothing beside it, and no product with -inf arises.
+template <typename T>
+__device__ __forceinline__ void add_vec(Sums& a, const uint4& u) {
+  constexpr int N = 16 / sizeof(T);
+  if (sizeof(T) == 2 && a.m > kLpFloor + 1000.f && a.m < INFINITY) {
+    const uint4 w = floored<T>(u);
+    const F2 scale = pack(kLog2e, kLog2e), minus_m = pack(-a.m, -a.m);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      const F2 y = mul2(add2(pair_of<T>(w, e), minus_m), scale);
+      const float2 v = unpack(y);
+      const F2 z = pack(ptx::ex2(v.x), ptx::ex2(v.y));
+      a.s = add2(a.s, z);
+      a.t = fma2(z, y, a.t);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) add_pair(a, pair_of<T>(u, e));
+  }
 }
 
 // Sums relative to one maximum.
@@ -155,7 +230,7 @@ struct RowSums {
 // a's sums with the reference moved to m >= a.m.
 __device__ __forceinline__ RowSums at_max(const RowSums& a, float m) {
   if (a.m == -INFINITY && a.s == 0.f) return RowSums{m, 0.f, 0.f};  // nothing but -inf seen
-  const float d = a.m - m, c = ptx::ex2(d * kLog2e);
+  const float d = (a.m - m) * kLog2e, c = ptx::ex2(d);
   return RowSums{m, a.s * c, moved(c, d, a.s, a.t)};
 }
 
@@ -170,25 +245,30 @@ struct LpParams {
   int vocab, top_k;
 };
 
+// NT: threads of a CTA.  A row to itself gets 256 (four CTAs on an SM: a row's serial end hides
+// behind three others' loads), a cluster's share 512.  [2048, 128256] bf16 takes 145 us with 256 and 152 with 512,
+// one row of it on 8 CTAs 8.4 and 7.4, 37 x 50,001 fp32 on 4 CTAs each 10.5 and 9.3.
+template <int NT>
 struct LpShared {
   unsigned long long keys[kLpBuf];
   unsigned long long best[kLpMaxK];  // this CTA's K best, in order
   RowSums sums;                      // and its part of the row's sums
   RowSums all_sums[8];
-  float part[kLpThreads / 32][2];
-  uint32_t group_max[32];
+  float part[NT / 32][2];
+  uint32_t group_max[32], at_k;
   int count, n_best;
-  int wsum[kLpThreads / 32];
+  int wsum[NT / 32];
 };
 
 // Sum of `c` over the CTA (two barriers).
-__device__ __forceinline__ int block_count(LpShared& sh, int c) {
+template <int NT>
+__device__ __forceinline__ int block_count(LpShared<NT>& sh, int c) {
   c = __reduce_add_sync(0xffffffffu, c);
   if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = c;
   __syncthreads();
   int t = 0;
 #pragma unroll
-  for (int i = 0; i < kLpThreads / 32; ++i) t += sh.wsum[i];
+  for (int i = 0; i < NT / 32; ++i) t += sh.wsum[i];
   __syncthreads();
   return t;
 }
@@ -197,14 +277,15 @@ __device__ __forceinline__ int block_count(LpShared& sh, int c) {
 // at its front in any order; keys of elements [drop_lo, drop_hi) are dropped
 // first.  Returns how many stay; *kth gets the smallest kept key (0 if
 // fewer than K).  Every thread of the CTA takes part.
-__device__ int keep_best(LpShared& sh, int K, int drop_lo, int drop_hi, unsigned long long* kth) {
+template <int NT>
+__device__ int keep_best(LpShared<NT>& sh, int K, int drop_lo, int drop_hi, unsigned long long* kth) {
   __syncthreads();
   const int n = min(sh.count, kLpBuf);
-  unsigned long long mine[kLpPerThread];
+  unsigned long long mine[(kLpBuf / NT)];
   int have = 0;
 #pragma unroll
-  for (int i = 0; i < kLpPerThread; ++i) {
-    const int at = threadIdx.x + i * kLpThreads;
+  for (int i = 0; i < (kLpBuf / NT); ++i) {
+    const int at = threadIdx.x + i * NT;
     unsigned long long k = at < n ? sh.keys[at] : 0ull;
     const int idx = (int)(0xffffffffu - (uint32_t)k);
     if (idx >= drop_lo && idx < drop_hi) k = 0ull;
@@ -220,7 +301,7 @@ __device__ int keep_best(LpShared& sh, int K, int drop_lo, int drop_hi, unsigned
       const unsigned long long mid = lo + ((hi - lo) >> 1);
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < kLpPerThread; ++i) c += mine[i] >= mid;
+      for (int i = 0; i < (kLpBuf / NT); ++i) c += mine[i] >= mid;
       c = block_count(sh, c);
       if (c >= K) {
         lo = mid;
@@ -233,7 +314,7 @@ __device__ int keep_best(LpShared& sh, int K, int drop_lo, int drop_hi, unsigned
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kLpPerThread; ++i)
+  for (int i = 0; i < (kLpBuf / NT); ++i)
     if (mine[i] >= lo) sh.keys[atomicAdd(&sh.count, 1)] = mine[i];
   __syncthreads();
   const int kept = sh.count;
@@ -262,53 +343,77 @@ __device__ __forceinline__ const P* of_cta(const P* x, uint32_t rank) {
 }
 
 // Sum and maximum over the CTA, the same in every thread.
-__device__ __forceinline__ float block_max(LpShared& sh, float x) {
+template <int NT>
+__device__ __forceinline__ float block_max(LpShared<NT>& sh, float x) {
   float w;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(w) : "f"(x));
   if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5][0] = w;
   __syncthreads();
   float m = sh.part[0][0];
 #pragma unroll
-  for (int i = 1; i < kLpThreads / 32; ++i) m = fmaxf(m, sh.part[i][0]);
+  for (int i = 1; i < NT / 32; ++i) m = fmaxf(m, sh.part[i][0]);
   __syncthreads();
   return m;
 }
 
+// The K-th largest of sh.group_max (0: fewer than K groups have anything); for the whole CTA, after
+// every group has put its maximum there.
+template <int NT>
+__device__ __forceinline__ uint32_t kth_of_groups(LpShared<NT>& sh, int K) {
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const uint32_t mine = sh.group_max[lane];
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+      above += other > mine || (other == mine && j < lane);
+    }
+    if (above == K - 1) sh.at_k = mine;
+  }
+  __syncthreads();
+  return sh.at_k;
+}
+
+// A value that K keys of the buffer at least reach (0: none found), by groups of keys.
+template <int NT>
+__device__ uint32_t reached_by_k(LpShared<NT>& sh, int K) {
+  const int tid = threadIdx.x;
+  if (tid < 32) sh.group_max[tid] = 0u;
+  __syncthreads();
+  const int n = min(sh.count, kLpBuf);
+  for (int i = tid; i < n; i += NT) atomicMax(&sh.group_max[i & 31], (uint32_t)(sh.keys[i] >> 32));
+  return kth_of_groups(sh, K);
+}
+
 // The K best keys of the buffer, in order, into sh.best; fewer if there are no more.
-__device__ void select_best(LpShared& sh, int K, unsigned long long* scratch_kth) {
+template <int NT>
+__device__ void select_best(LpShared<NT>& sh, int K, unsigned long long* scratch_kth) {
+  const int tid = threadIdx.x;
   __syncthreads();
   int n = sh.count;
-  const int tid = threadIdx.x;
-  if (n > 64) {
+  if (n > 32) {
+    const uint32_t least = n <= 2 * NT ? reached_by_k(sh, K) : 0u;
     bool few = false;
-    if (n <= kLpThreads) {
-      // one key a thread: bisection over the values alone, until at most 64 keys are left
-      const unsigned long long k = tid < n ? sh.keys[tid] : 0ull;
-      const uint32_t o = (uint32_t)(k >> 32);
-      uint32_t lo = 0u, hi = 0xffffffffu;  // count(o >= lo) >= K; the same below hi need not hold
-      while (!few && hi - lo > 1u) {
-        const uint32_t mid = lo + ((hi - lo) >> 1);
-        const int c = __syncthreads_count(tid < n && o >= mid);
-        if (c >= K) {
-          lo = mid;
-          few = c <= 64;
-        } else {
-          hi = mid;
-        }
-      }
-      if (few) {
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        if (tid < n && o >= lo) sh.keys[atomicAdd(&sh.count, 1)] = k;
-        __syncthreads();
-        n = sh.count;
-      }
+    if (least) {
+      const unsigned long long k0 = tid < n ? sh.keys[tid] : 0ull;
+      const unsigned long long k1 = tid + NT < n ? sh.keys[tid + NT] : 0ull;
+      const bool in0 = (uint32_t)(k0 >> 32) >= least, in1 = (uint32_t)(k1 >> 32) >= least;
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      if (in0) sh.keys[atomicAdd(&sh.count, 1)] = k0;
+      if (in1) sh.keys[atomicAdd(&sh.count, 1)] = k1;
+      __syncthreads();
+      n = sh.count;
+      few = n <= NT;  // many only where many are equal
     }
     if (!few) n = keep_best(sh, K, 0, 0, scratch_kth);
   }
   if (tid < n) {
     const unsigned long long k = sh.keys[tid];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += sh.keys[j] > k;
     if (rank < K) sh.best[rank] = k;
   }
@@ -316,11 +421,11 @@ __device__ void select_best(LpShared& sh, int K, unsigned long long* scratch_kth
 }
 
 // One cluster (of one CTA or more) per row.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpParams p) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpParams p) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
   constexpr int N = 16 / sizeof(T);
-  __shared__ LpShared sh;
+  __shared__ LpShared<NT> sh;
   const int K = p.top_k, V = p.vocab, tid = threadIdx.x, lane = tid & 31;
   const uint32_t ctas = cluster_size(), rank = blockIdx.x % ctas;
   const long long row = blockIdx.x / ctas;
@@ -358,76 +463,73 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     if (single >= 0) {
       const float f = DT<T>::to_f(x[single]);
       raise_max(a, f);
-      const float ref = a.m == -INFINITY ? 0.f : a.m;
-      add_pair(a, pack(f, -INFINITY), pack(-ref, -ref));
+      add_pair(a, pack(f, -INFINITY));
       if (K > 0) push(f, single);
     }
   }
 
-  for (int base = v0; base < v1; base += kLpThreads * kLpUnroll) {
-    uint4 u[kLpUnroll];
-    float vm[kLpUnroll];
-#pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
-      const int i = base + k * kLpThreads + tid;
-      if (i < v1) u[k] = __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
-    }
-    float tm = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
-      if (base + k * kLpThreads + tid < v1) {
-        vm[k] = vec_max<T>(u[k]);
-        tm = max_nan(tm, vm[k]);
-        if (!(vm[k] <= a.m)) raise_max(a, vm[k]);
-        const float ref = a.m == -INFINITY ? 0.f : a.m;
-        const F2 minus_m = pack(-ref, -ref);
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) add_pair(a, pair_of<T>(u[k], e), minus_m);
-      }
-    }
-    if (K == 0) continue;
-    if (base == v0) {
-      // The K-th largest of the maxima of 32 groups of 16 threads: K logits at least are not below it.
-      const uint32_t o = tid < v1 - v0 ? order_of(tm) : 0u;
-      const uint32_t top = __reduce_max_sync(lane < 16 ? 0x0000ffffu : 0xffff0000u, o);
-      if ((lane & 15) == 0) sh.group_max[tid >> 4] = top;
-      __syncthreads();
-      const uint32_t mine = sh.group_max[lane];
-      int above = 0;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
-        above += other > mine || (other == mine && j < lane);
-      }
-      const uint32_t at_k = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, above == K - 1)) - 1);
-      if (at_k) tau = value_of(at_k);  // 0: fewer than K groups have elements
-    }
+  for (int from = v0; from < v1; from += kLpSteps * kLpUnroll * NT) {
+    const int to = min(from + kLpSteps * kLpUnroll * NT, v1);
     bool full = false;
+    for (int base = from; base < to; base += kLpUnroll * NT) {
+      uint4 u[kLpUnroll];
+      float vm[kLpUnroll];
 #pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
-      const int i = base + k * kLpThreads + tid;
-      if (i < v1 && !(vm[k] < tau)) {
-        const T* h = reinterpret_cast<const T*>(&u[k]);
+      for (int k = 0; k < kLpUnroll; ++k) {
+        const int i = base + k * NT + tid;
+        if (i < to) u[k] = __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
+      }
+      float tm = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float f = DT<T>::to_f(h[e]);
-          if (!(f < tau)) full |= push(f, head + i * N + e);
+      for (int k = 0; k < kLpUnroll; ++k) {
+        if (base + k * NT + tid < to) {
+          vm[k] = vec_max<T>(u[k]);
+          tm = max_nan(tm, vm[k]);
+          if (!(vm[k] <= a.m + kLpSlack)) raise_max(a, vm[k]);
+          add_vec<T>(a, u[k]);
+        }
+      }
+      if (K == 0) continue;
+      if (base == v0) {
+        // The K-th largest of the maxima of 32 groups of threads: K logits at least are not below it.
+        const uint32_t o = tid < v1 - v0 ? order_of(tm) : 0u;
+        const uint32_t top = __reduce_max_sync(NT == 512 ? 0xffffu << (lane & 16) : 0xffu << (lane & 24), o);
+        if (tid % (NT / 32) == 0) sh.group_max[tid / (NT / 32)] = top;
+        const uint32_t at_k = kth_of_groups(sh, K);
+        if (at_k) tau = value_of(at_k);  // 0: fewer than K groups have elements
+      }
+#pragma unroll
+      for (int k = 0; k < kLpUnroll; ++k) {
+        const int i = base + k * NT + tid;
+        if (i < to && !(vm[k] < tau)) {
+          for (uint32_t bits = not_below<T>(u[k], tau); bits; bits &= bits - 1) {
+            const int e = __ffs(bits) - 1;
+            full |= push(DT<T>::to_f(element<T>(u[k], e)), head + i * N + e);
+          }
         }
       }
     }
-    if (!__syncthreads_or(full)) continue;
+    if (K == 0) continue;
+    if (!__syncthreads_or(full)) {
+      if (from == v0 && to < v1 && sh.count > 2 * K) {
+        const uint32_t least = reached_by_k(sh, K);
+        if (least) tau = value_of(least);
+        __syncthreads();
+      }
+      continue;
+    }
     if (sh.count <= kLpBuf) {
       keep_best(sh, K, 0, 0, &tau_key);
     } else {
-      // Keys of this tile were lost: take the tile out and push it again, one
-      // element a thread at a time, cutting back whenever the next step might overflow.
-      keep_best(sh, K, head + base * N, head + min(base + kLpThreads * kLpUnroll, v1) * N, &tau_key);
-      for (int k = 0; k < kLpUnroll; ++k) {
-        const int i = base + k * kLpThreads + tid;
+      // Keys of these steps were lost: take the steps out and push them again, one
+      // element a thread at a time, cutting back whenever the next push might overflow.
+      keep_best(sh, K, head + from * N, head + to * N, &tau_key);
+      for (int base = from; base < to; base += NT) {
+        const int i = base + tid;
         for (int e = 0; e < N; ++e) {
-          if (i < v1) push(DT<T>::to_f(xv[(size_t)i * N + e]), head + i * N + e);
+          if (i < to) push(DT<T>::to_f(xv[(size_t)i * N + e]), head + i * N + e);
           __syncthreads();
-          const bool cut = sh.count > kLpBuf - kLpThreads;
+          const bool cut = sh.count > kLpBuf - NT;
           __syncthreads();
           if (cut) keep_best(sh, K, 0, 0, &tau_key);
         }
@@ -437,7 +539,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     if (tau_key) tau = value_of((uint32_t)(tau_key >> 32));
   }
 
-  // This CTA's sums: the maximum first, then every thread's sums relative to it.
+  // This CTA's sums: the largest reference first, then every thread's sums relative to it.
   {
     const float m = block_max(sh, a.m);
     const float2 s2 = unpack(a.s), t2 = unpack(a.t);
@@ -456,7 +558,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     if (tid == 0) {
       s = t = 0.f;
 #pragma unroll
-      for (int i = 0; i < kLpThreads / 32; ++i) {
+      for (int i = 0; i < NT / 32; ++i) {
         s += sh.part[i][0];
         t += sh.part[i][1];
       }
@@ -492,7 +594,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     auto logprob = [&](float f) -> float { return (f - r.m) - log_s; };
     if (tid == 0) {
       p.logprobs[row] = inside ? logprob(x_tok) : -INFINITY;
-      p.entropy[row] = log_s - r.t / r.s;
+      p.entropy[row] = log_s - kLn2 * (r.t / r.s);
     }
     // The row's K best are those of all CTAs' K best that fewer than K others exceed.
     if (tid < n_all && sh.keys[tid] != 0ull) {
@@ -508,11 +610,11 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
   if (ctas > 1) cluster_sync();  // no CTA ends while its shared memory is read
 }
 
-template <typename T>
-cudaError_t launch_logprobs(const LpParams& p, int rows, int ctas, cudaStream_t stream) {
+template <typename T, int NT>
+cudaError_t launch_nt(const LpParams& p, int rows, int ctas, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * ctas);
-  cfg.blockDim = kLpThreads;
+  cfg.blockDim = NT;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -522,7 +624,18 @@ cudaError_t launch_logprobs(const LpParams& p, int rows, int ctas, cudaStream_t 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = tvk::pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p);
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, p);
+}
+
+// CTAs per row: as many as keep all rows resident at once, but none with less than a vector per
+// thread.  Two CTAs of 512 threads fit on each of 148 SMs, but clusters of 8 do not fill every GPC:
+// 37 fp32 rows of 50,001 take 14.6 us on 8 CTAs each (two waves) and 9.7 on 4.
+template <typename T>
+cudaError_t launch_logprobs(const LpParams& p, int rows, cudaStream_t stream) {
+  const long long vecs = (long long)p.vocab * (long long)sizeof(T) / 16;
+  int ctas = 8;
+  while (ctas > 1 && ((long long)rows * ctas > 256 || vecs < (long long)ctas * 512)) ctas >>= 1;
+  return ctas == 1 ? launch_nt<T, 256>(p, rows, 1, stream) : launch_nt<T, 512>(p, rows, ctas, stream);
 }
 
 }  // namespace
@@ -541,15 +654,10 @@ extern "C" int tvk_token_logprobs(const void* logits, const int32_t* tokens, flo
   TVK_CHECK_ARG((uintptr_t)logits % tvk::dtype_size(dtype) == 0, "logits must be aligned to their elements");
   const LpParams p{logits, tokens, logprobs, entropy, top_logprobs, top_tokens, row_stride, vocab, top_k};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // CTAs per row: as many as keep all rows resident at once (two CTAs on each of 148
-  // SMs), but none with less than a tile of its own.
-  const long long vecs = (long long)vocab * (long long)tvk::dtype_size(dtype) / 16;
-  int ctas = 8;
-  while (ctas > 1 && ((long long)rows * ctas > 296 || vecs < (long long)ctas * kLpThreads)) ctas >>= 1;
   switch (dtype) {
-    case TVK_DTYPE_F16: TVK_CHECK_CUDA(launch_logprobs<__half>(p, rows, ctas, s)); break;
-    case TVK_DTYPE_BF16: TVK_CHECK_CUDA(launch_logprobs<__nv_bfloat16>(p, rows, ctas, s)); break;
-    default: TVK_CHECK_CUDA(launch_logprobs<float>(p, rows, ctas, s)); break;
+    case TVK_DTYPE_F16: TVK_CHECK_CUDA(launch_logprobs<__half>(p, rows, s)); break;
+    case TVK_DTYPE_BF16: TVK_CHECK_CUDA(launch_logprobs<__nv_bfloat16>(p, rows, s)); break;
+    default: TVK_CHECK_CUDA(launch_logprobs<float>(p, rows, s)); break;
   }
   TVK_CHECK_LAUNCH("token_logprobs");
   return TVK_OK;
