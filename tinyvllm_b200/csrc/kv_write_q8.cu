@@ -11,15 +11,22 @@
 // the exponents of the codes already there; they lose nothing until they reach
 // e4m3's subnormals.  A call's last row for a slot wins, the others do not count.
 //
-// One CTA per token finds out whether its token is the first of the call in its
-// block (by reading all slots) and if so does the whole block, one warp per (K
-// or V, head), so no two CTAs write one block and nothing depends on their order.
+// A CTA looks after a few neighbouring tokens.  For each that might be the first of
+// the call in its block (the token before it lies in another) it reads all slots, which
+// says whether it is and which rows the block gets, and if so does the whole block,
+// one warp per (K or V, head).  So no two CTAs write one block and nothing depends on
+// their order, whatever the slots are; with prompts' runs of slots there is one
+// such token per block.  Reading all slots per block costs T^2 / block_size reads from L2: at 8,192
+// tokens about a third of the call (33 us for 50 MB of rows and codes), and what bounds calls of
+// more than some 30,000 rows.  Few tokens are latency: slot, other slots, rows, store, one
+// behind the other (64 rows of 4 heads of 64: 4.7 us, 256 of 8 of 128: 6.5 us).
 #include "kv_cache_q8.cuh"
 
 namespace {
 
 constexpr int kWriteThreads = 256;
 constexpr int kMaxBlockSize = 1024;
+constexpr int kFewTokens = 1024, kChunk = 16;  // tokens per CTA: one up to kFewTokens, else kChunk
 
 struct WriteParams {
   const void *k, *v;           // [n_tokens, n_kv_heads, head_dim]
@@ -27,27 +34,27 @@ struct WriteParams {
   float *k_scale, *v_scale;    // [num_blocks, n_kv_heads]
   const int64_t* slots;  // [n_tokens]
   int n_tokens, n_kv_heads, head_dim, block_size;
+  int chunk;  // tokens a CTA looks after
   long long n_slots;
 };
 
+// Eight elements as they lie in memory, and as floats.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* f) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x;
-    f[1] = a.y;
-    f[2] = a.z;
-    f[3] = a.w;
-    f[4] = b.x;
-    f[5] = b.y;
-    f[6] = b.z;
-    f[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = DT<T>::to_f(h[i]);
-  }
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void to_floats(const Raw8<T>& r, float* f) {
+  const T* h = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = DT<T>::to_f(h[i]);
 }
 
 __device__ __forceinline__ uint2 encode8(const float* f) {
@@ -57,79 +64,159 @@ __device__ __forceinline__ uint2 encode8(const float* f) {
   return c;
 }
 
+// Rows of D8 groups of 8 elements, walked 32 groups at a time by a warp.
+struct Walk8 {
+  int row, c, drow, dc, D8;
+  __device__ Walk8(int lane, int D8_) : row(lane / D8_), c(lane % D8_), drow(32 / D8_), dc(32 % D8_), D8(D8_) {}
+  __device__ void next() {
+    row += drow;
+    c += dc;
+    if (c >= D8) {
+      c -= D8;
+      ++row;
+    }
+  }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads) write_kv_q8_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const WriteParams p) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ int row_of[kMaxBlockSize];  // last token of the call for each slot of the block, or -1
-  __shared__ int first;
-  const int t = blockIdx.x, tid = threadIdx.x, bs = p.block_size;
-  const long long slot = p.slots[t];
-  if (slot < 0 || slot >= p.n_slots) return;
-  const long long blk = slot / bs, base = blk * bs;
-  if (t > 0) {  // the token before it is in the same block: not the first
-    const long long d = p.slots[t - 1] - base;
-    if (d >= 0 && d < bs) return;
-  }
-  for (int i = tid; i < bs; i += kWriteThreads) row_of[i] = -1;
-  if (tid == 0) first = t;
-  __syncthreads();
-  for (int i = tid; i < p.n_tokens; i += kWriteThreads) {
-    const long long d = p.slots[i] - base;
-    if (d >= 0 && d < bs) {
-      atomicMax(&row_of[d], i);
-      if (i < t) atomicMin(&first, i);
+  __shared__ int row_of[kMaxBlockSize];   // last token of the call for each slot of the block, or -1
+  __shared__ int2 rows[kMaxBlockSize];    // (slot in the block, token) of those there are
+  __shared__ int first, n_rows, cands[kChunk], n_cands;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bs = p.block_size;
+  const int D = p.head_dim, D8 = D / 8, H = p.n_kv_heads;
+  const size_t row_elems = (size_t)H * D;
+  if (tid < 32) {
+    // the chunk's tokens that the token before them does not share the block with
+    const int t = blockIdx.x * p.chunk + lane;
+    bool cand = false;
+    if (lane < p.chunk && t < p.n_tokens) {
+      const long long slot = p.slots[t], before = t > 0 ? p.slots[t - 1] : -1;
+      cand = slot >= 0 && slot < p.n_slots && (before < 0 || before / bs != slot / bs);
     }
+    const unsigned m = __ballot_sync(0xffffffffu, cand);
+    if (cand) cands[__popc(m & ((1u << lane) - 1u))] = t;
+    if (lane == 0) n_cands = __popc(m);
   }
   __syncthreads();
-  if (first != t) return;
-
-  const int warp = tid >> 5, lane = tid & 31;
-  const int D8 = p.head_dim / 8, H = p.n_kv_heads;
-  const bool started = row_of[0] >= 0;
-  for (int pair = blockIdx.y * (kWriteThreads / 32) + warp; pair < 2 * H; pair += gridDim.y * (kWriteThreads / 32)) {
-    const int kv = pair & 1, h = pair >> 1;
-    const T* x = reinterpret_cast<const T*>(kv ? p.v : p.k) + (size_t)h * p.head_dim;
-    uint8_t* codes = (kv ? p.v_cache : p.k_cache) + ((size_t)base * H + h) * p.head_dim;
-    float* sp = (kv ? p.v_scale : p.k_scale) + (size_t)blk * H + h;
-    float old = started ? 0.f : *sp;
-    if (!(old > 0.f && old < INFINITY)) old = 0.f;
-
-    float amax = 0.f;
-    for (int i = lane; i < bs * D8; i += 32) {
-      const int o = i / D8, c = i - o * D8;
-      const int r = row_of[o];
-      if (r < 0) continue;
-      float f[8];
-      load8<T>(x + (size_t)r * H * p.head_dim + c * 8, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (isfinite(f[e])) amax = fmaxf(amax, fabsf(f[e]));
+  for (int ci = 0; ci < n_cands; ++ci) {
+    const int t = cands[ci];
+    const long long blk = p.slots[t] / bs, base = blk * bs;
+    __syncthreads();  // the block before is done with
+    for (int i = tid; i < bs; i += kWriteThreads) row_of[i] = -1;
+    if (tid == 0) {
+      first = t;
+      n_rows = 0;
     }
+    __syncthreads();
+    auto look = [&](long long slot, int i) {
+      const unsigned long long d = (unsigned long long)(slot - base);
+      if (d < (unsigned long long)bs) {
+        atomicMax(&row_of[d], i);
+        if (i < t) atomicMin(&first, i);
+      }
+    };
+    // two slots a load where they are aligned (an odd last one apart)
+    const int pairs = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0 ? p.n_tokens / 2 : 0;
+#pragma unroll 8
+    for (int i = tid; i < pairs; i += kWriteThreads) {
+      const longlong2 two = reinterpret_cast<const longlong2*>(p.slots)[i];
+      look(two.x, 2 * i);
+      look(two.y, 2 * i + 1);
+    }
+    for (int i = 2 * pairs + tid; i < p.n_tokens; i += kWriteThreads) look(p.slots[i], i);
+    __syncthreads();
+    if (first != t) continue;  // the same for all threads
+    for (int i = tid; i < bs; i += kWriteThreads)
+      if (row_of[i] >= 0) rows[atomicAdd(&n_rows, 1)] = make_int2(i, row_of[i]);
+    __syncthreads();
+
+    const int n = n_rows;
+    const bool started = row_of[0] >= 0;
+    for (int pair = blockIdx.y * (kWriteThreads / 32) + warp; pair < 2 * H; pair += gridDim.y * (kWriteThreads / 32)) {
+      const int kv = pair & 1, h = pair >> 1;
+      const T* x = reinterpret_cast<const T*>(kv ? p.v : p.k) + (size_t)h * D;
+      uint8_t* codes = (kv ? p.v_cache : p.k_cache) + (size_t)base * row_elems + (size_t)h * D;
+      float* sp = (kv ? p.v_scale : p.k_scale) + (size_t)blk * H + h;
+      float old = started ? 0.f : *sp;
+      if (!(old > 0.f && old < INFINITY)) old = 0.f;
+
+      // Both passes read the rows; the second finds them in L1.
+      constexpr int kInFlight = 2;  // loads: more would cost the fourth CTA on an SM, which is worth more
+      auto for_rows = [&](auto&& use) {
+        Walk8 w(lane, D8);
+        while (w.row < n) {
+          Raw8<T> r[kInFlight];
+          int2 at[kInFlight];  // slot in the block (-1: none), group of 8
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float now = fmaxf(old, q8::scale_for(amax));
-    const float ratio = __fdiv_rn(old, now);
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *sp = now;
-    for (int i = lane; i < bs * D8; i += 32) {
-      const int o = i / D8, c = i - o * D8;
-      const int r = row_of[o];
-      uint2* dst = reinterpret_cast<uint2*>(codes + (size_t)o * H * p.head_dim + c * 8);
-      float f[8];
-      if (r >= 0) {
-        load8<T>(x + (size_t)r * H * p.head_dim + c * 8, f);
+          for (int k = 0; k < kInFlight; ++k) {
+            at[k].x = -1;
+            if (w.row < n) {
+              const int2 row = rows[w.row];
+              at[k] = make_int2(row.x, w.c);
+              r[k] = load8<T>(x + (size_t)row.y * row_elems + w.c * 8);
+            }
+            w.next();
+          }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = isfinite(f[e]) ? __fdiv_rn(f[e], now) : __int_as_float(0x7fffffff);
-        *dst = encode8(f);
-      } else if (started) {
-        *dst = make_uint2(0u, 0u);
-      } else if (now != old) {
-        const uint2 u = *dst;
-        q8::decode4(u.x, f);
-        q8::decode4(u.y, f + 4);
+          for (int k = 0; k < kInFlight; ++k)
+            if (at[k].x >= 0) use(r[k], at[k].x, at[k].y);
+        }
+      };
+      float amax = 0.f;
+      for_rows([&](const Raw8<T>& r, int, int) {
+        float f[8];
+        to_floats<T>(r, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= ratio;
-        *dst = encode8(f);
+        for (int e = 0; e < 8; ++e)
+          if (isfinite(f[e])) amax = fmaxf(amax, fabsf(f[e]));
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const float now = fmaxf(old, q8::scale_for(amax));
+      // Dividing by a power of two is multiplying by its reciprocal; other scales come from the caller only.
+      const uint32_t bits = __float_as_uint(now);
+      const bool pow2 = (bits & 0x7fffffu) == 0u && bits >= 0x00800000u && bits <= 0x7e800000u;
+      const float inv = pow2 ? __uint_as_float(0x7f000000u - bits) : 0.f;
+      __syncwarp();  // every lane has read the old scale
+      if (lane == 0) *sp = now;
+
+      for_rows([&](const Raw8<T>& r, int slot_in, int c) {
+        float f[8];
+        to_floats<T>(r, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = pow2 ? f[e] * inv : __fdiv_rn(f[e], now);
+          f[e] = isfinite(f[e]) ? y : __int_as_float(0x7fffffff);
+        }
+        *reinterpret_cast<uint2*>(codes + (size_t)slot_in * row_elems + c * 8) = encode8(f);
+      });
+
+      if (n < bs && (started || now != old)) {  // the block's other rows
+        const float ratio = __fdiv_rn(old, now);
+        Walk8 o(lane, D8);
+        while (o.row < bs) {
+          uint2 u[4];
+          uint2* dst[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bool other = o.row < bs && row_of[min(o.row, bs - 1)] < 0;
+            dst[k] = other ? reinterpret_cast<uint2*>(codes + (size_t)o.row * row_elems + o.c * 8) : nullptr;
+            u[k] = other && !started ? *dst[k] : make_uint2(0u, 0u);
+            o.next();
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (!dst[k]) continue;
+            float f[8];
+            q8::decode4(u[k].x, f);
+            q8::decode4(u[k].y, f + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= ratio;
+            *dst[k] = started ? make_uint2(0u, 0u) : encode8(f);
+          }
+        }
       }
     }
   }
@@ -145,8 +232,7 @@ extern "C" int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t
   TVK_CHECK_ARG(n_tokens >= 0, "negative n_tokens");
   TVK_CHECK_ARG(n_kv_heads > 0 && num_blocks > 0 && block_size > 0, "sizes must be positive");
   TVK_CHECK_ARG(head_dim > 0 && head_dim % 16 == 0, "head_dim must be a multiple of 16 (got %d)", head_dim);
-  TVK_CHECK_ARG((long long)block_size * head_dim < 0x7fffffffLL && (long long)n_kv_heads * head_dim < 0x7fffffffLL,
-                "a block's rows exceed the 32-bit index");
+  TVK_CHECK_ARG(head_dim <= 65536 && n_kv_heads <= 65536, "head_dim and n_kv_heads must be at most 65536");
   TVK_CHECK_ARG(dtype == TVK_DTYPE_F32 || dtype == TVK_DTYPE_F16 || dtype == TVK_DTYPE_BF16, "unknown dtype %d", dtype);
   if (block_size > kMaxBlockSize) {
     tvk::set_error("block_size %d unsupported (at most %d)", block_size, kMaxBlockSize);
@@ -157,8 +243,9 @@ extern "C" int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t
   TVK_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_cache) && aligned16(v_cache),
                 "k, v, k_cache and v_cache must be 16-byte aligned");
   const WriteParams p{k, v, (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, slots, n_tokens, n_kv_heads,
-                      head_dim, block_size, (long long)num_blocks * block_size};
-  const dim3 grid(n_tokens, 1);
+                      head_dim, block_size, n_tokens > kFewTokens ? kChunk : 1, (long long)num_blocks * block_size};
+  // a warp per (K or V, head)
+  const dim3 grid((n_tokens + p.chunk - 1) / p.chunk, (2 * n_kv_heads + kWriteThreads / 32 - 1) / (kWriteThreads / 32));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
     case TVK_DTYPE_F16: TVK_CHECK_CUDA(tvk::launch_pdl(write_kv_q8_kernel<__half>, grid, kWriteThreads, 0, s, p)); break;
