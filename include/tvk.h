@@ -44,6 +44,12 @@ int tvk_abi_version(void);
 const char* tvk_last_error(void);
 
 /*
+ * Id of the capture that `stream` is recording, 0 if it is not capturing, into *id (host
+ * memory).  For callers that give every captured graph a workspace of its own.
+ */
+int tvk_stream_capture_id(unsigned long long* id, void* stream);
+
+/*
  * Bytes of scratch that tvk_paged_decode_attention needs for a batch whose
  * block tables are `max_blocks` wide: a 256-byte header (a device status word
  * at byte 0, work-list counters at bytes 64 and 128, the unit size of the last
@@ -272,10 +278,11 @@ int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t* slots, vo
 /*
  * Bytes of scratch tvk_paged_decode_attention_q8 needs: a 256-byte header (the
  * status word at byte 0), a fixed area for the partial sums of sequences that
- * several CTAs share, and one arrival counter per (sequence, KV head).  Zero all
- * of it once; every call leaves header and counters zero (the status word only if
- * no kernel wait timed out).  One workspace serves one stream at a time and is
- * not shared with other entry points.
+ * several CTAs share, and behind it arrival counters, four per (sequence, KV head).
+ * Zero header and counters (or all of it) once; every call leaves them zero (the status
+ * word only if no kernel wait timed out), whatever its sizes.  One workspace serves one stream at a
+ * time (two captured graphs that may run at once need one each) and is not shared with
+ * other entry points.
  */
 size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads);
 

@@ -354,3 +354,38 @@ def test_two_streams_and_captured_graphs(cuda):
         other = _run(cs[1])
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(other, want[1])
+
+
+def test_two_graphs_recorded_on_one_stream_replay_at_once(cuda):
+    """Each recorded graph has a workspace of its own: both split their sequences over CTAs, and run on two streams."""
+    cs = [_case(cuda, B, 32, 8, 128, 16, ctx, torch.bfloat16, s) for s, B, ctx in ((1, 3, [5000, 700, 9000]), (2, 40, [3000] * 40))]
+    want = [_run(c).clone() for c in cs]
+    outs, graphs = [torch.empty_like(w) for w in want], []
+    rec = torch.cuda.Stream()
+    for c, o in zip(cs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=rec):
+            for _ in range(3):
+                _run(c, out=o)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_wait_that_runs_out_is_told_and_the_next_call_is_right(cuda):
+    """The producers issue nothing (test hook): the kernel's waits run out, it says so and returns."""
+    from tinyvllm_b200 import _lib
+    from tinyvllm_b200.attention import workspace_status
+    c = _case(cuda, 6, 32, 8, 128, 16, [5, 70, 300, 900, 1500, 21000], torch.float16, 41)
+    want = _run(c, check=True).clone()
+    assert _lib.lib().tvk_debug_arm_wait_timeout(5_000_000) == 0
+    with pytest.raises(_lib.TvkError, match="timed out"):
+        _run(c, check=True)
+    assert workspace_status(cuda, "decode_q8") == 0
+    assert torch.equal(_run(c, check=True), want)

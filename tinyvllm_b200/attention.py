@@ -9,6 +9,7 @@ current torch stream.
 
 from __future__ import annotations
 
+import ctypes
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -33,6 +34,41 @@ def _workspace(device: torch.device, nbytes: int, kind: str = "decode") -> torch
         return ws
 
 
+_capture_workspaces: Dict[tuple, torch.Tensor] = {}
+
+
+def _capture_workspace(device: torch.device, nbytes: int, kind: str, zero_tail: int) -> Optional[torch.Tensor]:
+    """While the current stream records a CUDA graph: a workspace of that graph alone, so that
+    graphs recorded on one stream may run at the same time.  Its header and last
+    ``zero_tail`` bytes are zeroed by the graph itself at every replay.  It lives as long
+    as the process, as the per-stream workspaces do.  None while nothing is recorded."""
+    if not torch.cuda.is_current_stream_capturing():
+        return None
+    capture = ctypes.c_ulonglong()
+    rc = _lib.lib().tvk_stream_capture_id(ctypes.byref(capture), _lib.stream_ptr(device))
+    _lib.check(rc, "tvk_stream_capture_id")
+    if capture.value == 0:               # another device's stream is the one that records
+        return None
+    key = (device.index, capture.value, kind)
+    with _ws_lock:
+        ws = _capture_workspaces.get(key)
+        if ws is None or ws.numel() < nbytes:
+            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            ws[:256].zero_()
+            if zero_tail:
+                ws[ws.numel() - zero_tail:].zero_()
+            _capture_workspaces.setdefault((*key, ws.data_ptr()), ws)     # what a replay uses is never freed
+            _capture_workspaces[key] = ws
+        return ws
+
+
+def _workspace_q8(device: torch.device, batch: int, n_kv_heads: int) -> torch.Tensor:
+    L = _lib.lib()
+    nbytes = L.tvk_paged_decode_q8_workspace_size(batch, n_kv_heads)
+    ws = _capture_workspace(device, nbytes, "decode_q8", nbytes - L.tvk_paged_decode_q8_workspace_size(0, 0))
+    return _workspace(device, nbytes, "decode_q8") if ws is None else ws
+
+
 def workspace_status(device: Optional[torch.device] = None, kind: str = "decode") -> int:
     """Status word of the current stream's workspace (non-zero: a kernel wait timed out)."""
     device = device or torch.device("cuda", torch.cuda.current_device())
@@ -44,7 +80,8 @@ def status_word(device: Optional[torch.device] = None, kind: str = "decode") -> 
     """The current stream's workspace status word as a one-element int32 device tensor
     (a view: a CUDA graph can copy it out alongside its results)."""
     device = device or torch.device("cuda", torch.cuda.current_device())
-    return _workspace(device, 0, kind)[:4].view(torch.int32)
+    ws = _capture_workspace(device, 0, kind, 0) if kind == "decode_q8" else None
+    return (_workspace(device, 0, kind) if ws is None else ws)[:4].view(torch.int32)
 
 
 def check_workspace(device: Optional[torch.device] = None, kind: str = "decode", what: str = "kernel") -> None:
@@ -152,7 +189,7 @@ def paged_decode_attention_q8(queries: torch.Tensor, k_cache: torch.Tensor, v_ca
           or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor like queries")
     L = _lib.lib()
-    ws = _workspace(dev, L.tvk_paged_decode_q8_workspace_size(B, n_kv_heads), "decode_q8")
+    ws = _workspace_q8(dev, B, n_kv_heads)
     rc = _lib.call_on(
         dev, L.tvk_paged_decode_attention_q8, queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),

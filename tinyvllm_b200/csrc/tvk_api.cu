@@ -59,4 +59,13 @@ extern "C" int tvk_debug_arm_wait_timeout(long long limit_ns) {
   return TVK_OK;
 }
 
+extern "C" int tvk_stream_capture_id(unsigned long long* id, void* stream) {
+  TVK_CHECK_ARG(id, "null id pointer");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long of = 0;
+  TVK_CHECK_CUDA(cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &of));
+  *id = status == cudaStreamCaptureStatusActive ? of : 0;
+  return TVK_OK;
+}
+
 extern "C" const char* tvk_last_error(void) { return tvk::g_last_error; }

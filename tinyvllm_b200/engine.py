@@ -20,6 +20,11 @@ iterations (engine.py:114-196), blocks freed when a sequence finishes
   128), the latter over a token buffer whose tail is a padding prompt that
   stores nothing; up to 64 prefill graphs are kept, further shapes run eagerly.
 
+``kv_cache_dtype="float8_e4m3fn"`` keeps the K/V cache in 8 bits with one scale per block
+and KV head (half the bytes of a 16-bit cache; no counterpart in the reference).
+``SamplingParams.logprobs = n`` returns for each sampled token its log probability, the
+entropy of its distribution and the n most likely tokens, from the step's logits.
+
 ``kv_order="reference"`` (default) reproduces the reference decode exactly:
 tables padded / truncated to 64 blocks (engine.py:81, llama.py:368-374),
 attention over ``position + 1`` slots before the step's own K/V is written.
@@ -31,7 +36,7 @@ from __future__ import annotations
 import time
 from dataclasses import dataclass, field
 from enum import Enum, auto
-from typing import Any, Callable, Dict, Iterator, List, Optional
+from typing import Any, Callable, Dict, Iterator, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -51,12 +56,24 @@ _MAX_PREFILL_GRAPHS = 64
 
 @dataclass
 class SamplingParams:
-    """core/sampling.py:12-18.  Only greedy decoding (temperature < 1e-5) is run here."""
+    """core/sampling.py:12-18.  Only greedy decoding (temperature < 1e-5) is run here.
+    ``logprobs``: None, or how many most likely tokens (0 to 32) to report with each
+    token's log probability."""
     temperature: float = 0.0
     top_k: int = 40
     top_p: float = 0.95
     repetition_penalty: float = 1.0
     max_tokens: int = 1024
+    logprobs: Optional[int] = None
+
+
+@dataclass
+class SampledLogprobs:
+    """What ``SamplingParams.logprobs`` asks for, of one sampled token (natural logarithms)."""
+    token: int
+    logprob: float
+    entropy: float
+    top: List[Tuple[int, float]]      # (token, log probability), most likely first
 
 
 class SequenceStatus(Enum):
@@ -72,6 +89,8 @@ class Sequence:
     prompt_tokens: List[int]
     output_tokens: List[int] = field(default_factory=list)
     status: SequenceStatus = SequenceStatus.WAITING
+    # one entry per output token where asked for (None: a first token that was given, not sampled)
+    logprobs: Optional[List[Optional[SampledLogprobs]]] = None
 
     def get_all_tokens(self) -> List[int]:
         return self.prompt_tokens + self.output_tokens
@@ -114,6 +133,7 @@ class GenerationOutput:
     text: str
     tokens: List[int]
     finish_reason: str  # 'eos', 'length' or 'abort'
+    logprobs: Optional[List[Optional[SampledLogprobs]]] = None   # as SamplingParams.logprobs asks for
 
 
 class Scheduler:
@@ -139,7 +159,8 @@ class Scheduler:
             request = self.waiting.pop(0)
             self.block_manager.register_sequence(self.next_seq_id, self.gpu_id)
             seq = Sequence(self.next_seq_id, request.request_id, request.prompt_tokens,
-                           status=SequenceStatus.RUNNING)
+                           status=SequenceStatus.RUNNING,
+                           logprobs=None if request.sampling_params.logprobs is None else [])
             request.sequence = seq
             self.next_seq_id += 1
             self.running[seq.seq_id] = seq
@@ -191,9 +212,11 @@ class LLMEngine:
                  block_size: int = 16, num_scheduler_steps: int = 1, kv_order: str = "reference",
                  max_table_blocks: Optional[int] = None, gpu_id: int = 0,
                  output_callback: Optional[Callable[[GenerationOutput], None]] = None,
-                 use_cuda_graphs: bool = False):
+                 use_cuda_graphs: bool = False, kv_cache_dtype: Optional[str] = None):
         if kv_order not in ("reference", "append_first"):
             raise ValueError("kv_order must be 'reference' or 'append_first'")
+        if kv_cache_dtype not in (None, "float8_e4m3fn"):
+            raise ValueError("kv_cache_dtype must be None (the model's dtype) or 'float8_e4m3fn'")
         self.model = model
         self.tokenizer = tokenizer or TokenIdTokenizer()
         self.max_batch_size = max_batch_size
@@ -207,7 +230,7 @@ class LLMEngine:
         self.block_manager = BlockManager(num_gpus=gpu_id + 1, blocks_per_gpu=num_blocks, block_size=block_size)
         self.gpu_id = gpu_id
         self.kv_cache = KVCache(cfg.n_layers, num_blocks, block_size, cfg.n_kv_heads, cfg.head_dim,
-                                cfg.torch_dtype, self.device)
+                                cfg.torch_dtype if kv_cache_dtype is None else torch.float8_e4m3fn, self.device)
         self.scheduler = Scheduler(max_batch_size, self.block_manager, gpu_id)
         self.next_request_id = 0
         self.requests: Dict[int, Request] = {}
@@ -230,6 +253,8 @@ class LLMEngine:
         sp = sampling_params or SamplingParams()
         if sp.temperature >= _SAMPLING_EPS:
             raise ValueError("only greedy decoding (temperature < 1e-5) is supported by this engine")
+        if sp.logprobs is not None and not 0 <= sp.logprobs <= min(32, self.model.config.vocab_size):
+            raise ValueError("logprobs must be None or from 0 to 32 (and no more than the vocabulary)")
         tokens = self.tokenizer.encode(prompt)
         if not tokens:
             raise ValueError("empty prompt")
@@ -297,7 +322,8 @@ class LLMEngine:
             for rid, req in list(self.requests.items()):
                 if req.sequence is not None and req.sequence.seq_id == sid:
                     out = GenerationOutput(rid, self.tokenizer.decode(req.sequence.output_tokens),
-                                           list(req.sequence.output_tokens), self._reason(req.sequence))
+                                           list(req.sequence.output_tokens), self._reason(req.sequence),
+                                           req.sequence.logprobs)
                     outs.append(out)
                     if self.output_callback:
                         self.output_callback(out)
@@ -325,6 +351,8 @@ class LLMEngine:
                 bm.slot_mapping(s.seq_id, 0, s.get_prompt_len())
                 bm.advance_position(s.seq_id, s.get_prompt_len())
                 first[s.seq_id] = tok
+                if s.logprobs is not None:
+                    s.logprobs.append(None)
         if live:
             for s, t in zip(live, self._prefill_live(live)):
                 first[s.seq_id] = t
@@ -348,6 +376,7 @@ class LLMEngine:
                 graph = self.model.capture_prefill(n, t_pad, self.kv_cache, self._prefill_pool, self._prefill_stream)
                 self._prefill_graphs[(n, t_pad)] = graph
             sampled = graph.run(toks, pos, lens, slots).tolist()   # raises if a kernel wait timed out
+            self._add_logprobs(graph.logits, graph.out[:n], seqs)
         else:
             logits = self.model.prefill(torch.from_numpy(toks).to(dev), torch.from_numpy(pos).to(dev),
                                         torch.from_numpy(cu).to(dev), max(lens), torch.from_numpy(slots).to(dev),
@@ -388,6 +417,7 @@ class LLMEngine:
                 self._graphs[cap] = graph
             toks = np.asarray([s.output_tokens[-1] for s in seqs], dtype=np.int32)
             sampled = graph.run(toks, pos, bt, ctx, slots).tolist()
+            self._add_logprobs(graph.logits[:B], graph.out[:B], seqs)
         else:
             dev = self.device
             tok = torch.tensor([s.output_tokens[-1] for s in seqs], dtype=torch.int32, device=dev)
@@ -397,7 +427,7 @@ class LLMEngine:
             sampled = None
         if sampled is None:
             sampled = self._sample(logits, seqs)
-            check_workspace(self.device, "decode", "decode step")
+            check_workspace(self.device, self.kv_cache.decode_kind, "decode step")
         for i in ids:
             bm.advance_position(i)
         self.stats["decode_tokens"] += len(seqs)
@@ -406,7 +436,24 @@ class LLMEngine:
 
     def _sample(self, logits: torch.Tensor, seqs: List[Sequence]) -> List[int]:
         """Greedy pick for each row of ``logits`` [len(seqs), vocab] (sampling.py:133-134)."""
-        return layers.greedy_argmax(logits).cpu().tolist()
+        tokens = layers.greedy_argmax(logits)
+        self._add_logprobs(logits, tokens, seqs)
+        return tokens.cpu().tolist()
+
+    def _add_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, seqs: List[Sequence]) -> None:
+        """Log probabilities of this step's ``tokens`` (int32, one per row of ``logits``) for
+        the sequences that asked for them: one call over all rows, read back once."""
+        want = [self.requests[s.request_id].sampling_params.logprobs for s in seqs]
+        n = max((w for w in want if w is not None), default=None)
+        if n is None:
+            return
+        r = layers.token_logprobs(logits, tokens, n)
+        host = torch.cat([tokens[:, None].double(), r.logprobs[:, None].double(), r.entropy[:, None].double(),
+                          r.top_tokens.double(), r.top_logprobs.double()], dim=1).tolist()
+        for s, w, row in zip(seqs, want, host):
+            if w is not None:
+                top = [(int(t), lp) for t, lp in zip(row[3:3 + w], row[3 + n:3 + n + w])]
+                s.logprobs.append(SampledLogprobs(int(row[0]), row[1], row[2], top))
 
 
 def generate_batch(engine: LLMEngine, prompts: List, sampling_params: Optional[SamplingParams] = None) -> List[str]:

@@ -17,6 +17,10 @@ which attends over the cache *before* the step's own K/V is written
 (llama.py:328-332 then 381-386) with block tables built before the new slot is
 allocated (engine.py:247, llama.py:383); ``"append_first"`` writes the step's
 K/V first, so the query also sees its own key.
+
+With an 8-bit cache (``KVCache(..., torch.float8_e4m3fn)``) the same steps run over
+e4m3 codes with one scale per block and KV head: prompts attend over their own 16- or
+32-bit K/V and store it quantised, decode attends over the codes.
 """
 
 from __future__ import annotations
@@ -29,7 +33,8 @@ import numpy as np
 import torch
 
 from . import _lib, layers
-from .attention import flash_prefill_attention_varlen, paged_decode_attention, status_word
+from .attention import (flash_prefill_attention_varlen, paged_decode_attention, paged_decode_attention_q8,
+                        status_word)
 
 _DTYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -87,7 +92,9 @@ class LayerWeights:
 
 class KVCache:
     """Per-layer K and V pools ``[num_blocks, block_size, n_kv_heads, head_dim]``,
-    zero-initialised (core/kv_cache.py:13-32), as device tensors."""
+    zero-initialised (core/kv_cache.py:13-32), as device tensors.  With ``dtype``
+    ``torch.float8_e4m3fn`` the pools hold codes and ``k_scale`` / ``v_scale`` one fp32
+    scale per block and KV head (a value is code * scale)."""
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int,
                  dtype: torch.dtype, device="cuda"):
@@ -100,27 +107,63 @@ class KVCache:
         shape = (num_blocks, block_size, n_kv_heads, head_dim)
         self.k_cache = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
         self.v_cache = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.quantized = dtype == torch.float8_e4m3fn
+        n_scales = num_layers if self.quantized else 0
+        self.k_scale = [torch.zeros(num_blocks, n_kv_heads, device=device) for _ in range(n_scales)]
+        self.v_scale = [torch.zeros(num_blocks, n_kv_heads, device=device) for _ in range(n_scales)]
+
+    @property
+    def decode_kind(self) -> str:
+        """Which decode workspace attention over this cache uses."""
+        return "decode_q8" if self.quantized else "decode"
+
+    def write_slots(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Rows k, v [n, Hkv, D] at flat slots (int64 [n]; negative ones are skipped)."""
+        kc, vc = self.k_cache[layer_idx], self.v_cache[layer_idx]
+        if self.quantized:
+            layers.write_kv_slots_q8(k, v, slots, kc, vc, self.k_scale[layer_idx], self.v_scale[layer_idx])
+        else:
+            layers.write_kv_slots(k, v, slots, kc, vc)
+
+    def attend(self, layer_idx: int, q: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+               n_heads: int) -> torch.Tensor:
+        """Decode attention of q [B, 1, n_heads, D] over one layer of this cache."""
+        kc, vc = self.k_cache[layer_idx], self.v_cache[layer_idx]
+        if self.quantized:
+            return paged_decode_attention_q8(q, kc, vc, self.k_scale[layer_idx], self.v_scale[layer_idx], block_tables,
+                                             context_lens, n_heads, self.n_kv_heads, self.head_dim, self.block_size)
+        return paged_decode_attention(q, kc, vc, block_tables, context_lens, n_heads, self.n_kv_heads, self.head_dim,
+                                      self.block_size)
 
     def write_kv(self, layer_idx: int, block_id: int, start_offset: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """KVCache.write_kv (kv_cache.py:34-38): rows [n, Hkv, D] at ``block_id`` from ``start_offset``."""
         n = k.shape[0]
         slots = torch.arange(block_id * self.block_size + start_offset,
                              block_id * self.block_size + start_offset + n, dtype=torch.int64, device=k.device)
-        layers.write_kv_slots(k.contiguous(), v.contiguous(), slots, self.k_cache[layer_idx], self.v_cache[layer_idx])
+        self.write_slots(layer_idx, k.contiguous(), v.contiguous(), slots)
 
     def read_kv_blocks(self, layer_idx: int, block_ids: List[int], context_len: int):
-        """kv_cache.py:40-55 (test helper): [context_len, Hkv, D] gathered from ``block_ids``."""
+        """kv_cache.py:40-55 (test helper): [context_len, Hkv, D] gathered from ``block_ids``
+        (of an 8-bit cache the fp32 values)."""
         if not block_ids:
-            z = torch.zeros(0, self.n_kv_heads, self.head_dim, dtype=self.dtype, device=self.k_cache[0].device)
+            z = torch.zeros(0, self.n_kv_heads, self.head_dim, dtype=torch.float32 if self.quantized else self.dtype,
+                            device=self.k_cache[0].device)
             return z, z.clone()
         idx = torch.tensor(block_ids, dtype=torch.int64, device=self.k_cache[0].device)
+        if self.quantized:
+            def values(codes, scale):
+                x = codes.view(torch.uint8)[idx].view(torch.float8_e4m3fn).float() * scale[idx][:, None, :, None]
+                return x.reshape(-1, self.n_kv_heads, self.head_dim)[:context_len]
+            return (values(self.k_cache[layer_idx], self.k_scale[layer_idx]),
+                    values(self.v_cache[layer_idx], self.v_scale[layer_idx]))
         k = self.k_cache[layer_idx][idx].reshape(-1, self.n_kv_heads, self.head_dim)
         v = self.v_cache[layer_idx][idx].reshape(-1, self.n_kv_heads, self.head_dim)
         return k[:context_len], v[:context_len]
 
     def get_memory_bytes(self) -> int:
+        scales = 2 * 4 * self.num_layers * self.num_blocks * self.n_kv_heads if self.quantized else 0
         return (self.num_layers * self.num_blocks * self.block_size * self.n_kv_heads * self.head_dim * 2
-                * torch.tensor([], dtype=self.dtype).element_size())
+                * torch.tensor([], dtype=self.dtype).element_size()) + scales
 
 
 class Llama:
@@ -204,8 +247,12 @@ class Llama:
         x = layers.rms_norm(h, self.layers[0].attention_norm, c.norm_eps)
         for i, L in enumerate(self.layers):
             q, k, v = self._qkv(L, x, positions)
-            attn = flash_prefill_attention_varlen(q, k, v, cu_seqlens, max_seqlen, True, slot_mapping=slot_mapping,
-                                                  k_cache=kv_cache.k_cache[i], v_cache=kv_cache.v_cache[i])
+            if kv_cache.quantized:
+                attn = flash_prefill_attention_varlen(q, k, v, cu_seqlens, max_seqlen, True)
+                kv_cache.write_slots(i, k, v, slot_mapping)
+            else:
+                attn = flash_prefill_attention_varlen(q, k, v, cu_seqlens, max_seqlen, True, slot_mapping=slot_mapping,
+                                                      k_cache=kv_cache.k_cache[i], v_cache=kv_cache.v_cache[i])
             nxt = self.layers[i + 1].attention_norm if i + 1 < c.n_layers else self.norm
             x = self._layer_ffn(L, h, attn, nxt, T)
         last = (cu_seqlens[1:] if n_out is None else cu_seqlens[1:n_out + 1]) - 1
@@ -239,15 +286,23 @@ class Llama:
         x = layers.rms_norm(h, self.layers[0].attention_norm, c.norm_eps)
         for i, L in enumerate(self.layers):
             kc, vc = kv_cache.k_cache[i], kv_cache.v_cache[i]
-            if kv_order == "append_first":
+            append_first = kv_order == "append_first"
+            if append_first and not kv_cache.quantized:
                 q, k, v = self._qkv(L, x, positions, slots, kv_cache, i)
             else:
                 q, k, v = self._qkv(L, x, positions)
-            attn = paged_decode_attention(q.view(B, 1, c.n_heads, c.head_dim), kc, vc, block_tables, context_lens,
-                                          c.n_heads, c.n_kv_heads, c.head_dim, kv_cache.block_size)
+                if append_first:
+                    kv_cache.write_slots(i, k, v, slots)
+            attn = kv_cache.attend(i, q.view(B, 1, c.n_heads, c.head_dim), block_tables, context_lens, c.n_heads)
             # reference order: the new token's K/V reaches the pool after the attention
-            # (llama.py:381-386), stored by the launch of the norm that follows wo
-            late_kv = (k, v, slots, kc, vc) if kv_order != "append_first" else None
+            # (llama.py:381-386), stored by the launch of the norm that follows wo (an 8-bit
+            # cache's by its own)
+            late_kv = None
+            if not append_first:
+                if kv_cache.quantized:
+                    kv_cache.write_slots(i, k, v, slots)
+                else:
+                    late_kv = (k, v, slots, kc, vc)
             nxt = self.layers[i + 1].attention_norm if i + 1 < c.n_layers else self.norm
             x = self._layer_ffn(L, h, attn, nxt, B, write_kv=late_kv)
         return torch.matmul(x, self.output)
@@ -295,10 +350,11 @@ class DecodeGraph:
 
     def _forward(self):
         logits = self.model.decode(self.tok, self.pos, self.bt, self.ctx, self.slots, self.kv_cache, self.kv_order)
+        self.logits = logits    # of the last replay; its rows stay until the next one
         layers.greedy_argmax(logits, out=self.out[:self.batch])
         # the attention calls of this step used this stream's workspace; the view
         # also keeps that workspace alive for as long as the graph exists
-        self._status = status_word(self.model.device, "decode")
+        self._status = status_word(self.model.device, self.kv_cache.decode_kind)
         self.out[self.batch:].copy_(self._status)
 
     def run(self, tokens: np.ndarray, positions: np.ndarray, tables: np.ndarray, ctx: np.ndarray,
@@ -407,6 +463,7 @@ class PrefillGraph:
     def _forward(self):
         m = self.model
         logits = m.prefill(self.tok, self.pos, self.cu, self.T, self.slots, self.kv_cache, n_out=self.n)
+        self.logits = logits    # of the last replay; its rows stay until the next one
         layers.greedy_argmax(logits, out=self.out[:self.n])
         # the attention calls used this stream's prefill workspace; the view keeps it
         # alive for as long as the graph exists
