@@ -108,6 +108,20 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """``stream_ptr`` of device ``index``, without making a Stream object (a microsecond less per call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def same_device(*tensors: torch.Tensor) -> int:
+    """Index of the CUDA device that all tensors live on; raises as ``require_cuda`` does."""
+    index = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
+    for t in tensors:
+        if index < 0 or not isinstance(t, torch.Tensor) or t.get_device() != index:
+            return require_cuda(*tensors).index
+    return index
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = None
     for t in tensors:
@@ -120,10 +134,10 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-def call_on(dev: torch.device, fn, *args) -> int:
-    """``fn(*args)`` with ``dev`` as the current device (launches go to the current
-    device's context, and the tensors may live on another one)."""
-    if dev.index == torch.cuda.current_device():
+def call_on(index: int, fn, *args) -> int:
+    """``fn(*args)`` with device ``index`` as the current one (launches go to the current
+    device's context, and the tensors may live on another)."""
+    if index == torch.cuda.current_device():
         return fn(*args)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(index):
         return fn(*args)

@@ -37,7 +37,7 @@ def _workspace(device: torch.device, nbytes: int, kind: str = "decode") -> torch
 _capture_workspaces: Dict[tuple, torch.Tensor] = {}
 
 
-def _capture_workspace(device: torch.device, nbytes: int, kind: str, zero_tail: int) -> Optional[torch.Tensor]:
+def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Optional[torch.Tensor]:
     """While the current stream records a CUDA graph: a workspace of that graph alone, so that
     graphs recorded on one stream may run at the same time.  Its header and last
     ``zero_tail`` bytes are zeroed by the graph itself at every replay.  It lives as long
@@ -45,28 +45,39 @@ def _capture_workspace(device: torch.device, nbytes: int, kind: str, zero_tail: 
     if not torch.cuda.is_current_stream_capturing():
         return None
     capture = ctypes.c_ulonglong()
-    rc = _lib.lib().tvk_stream_capture_id(ctypes.byref(capture), _lib.stream_ptr(device))
+    rc = _lib.lib().tvk_stream_capture_id(ctypes.byref(capture), _lib.raw_stream(index))
     _lib.check(rc, "tvk_stream_capture_id")
     if capture.value == 0:               # another device's stream is the one that records
         return None
-    key = (device.index, capture.value, kind)
+    key = (index, capture.value, kind)
     with _ws_lock:
         ws = _capture_workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
             ws[:256].zero_()
             if zero_tail:
                 ws[ws.numel() - zero_tail:].zero_()
-            _capture_workspaces.setdefault((*key, ws.data_ptr()), ws)     # what a replay uses is never freed
+            _capture_workspaces[(*key, ws.data_ptr())] = ws     # what a replay uses is never freed
             _capture_workspaces[key] = ws
         return ws
 
 
-def _workspace_q8(device: torch.device, batch: int, n_kv_heads: int) -> torch.Tensor:
+_q8_fixed_bytes = 0
+
+
+def _workspace_q8(index: int, batch: int, n_kv_heads: int) -> torch.Tensor:
+    """The workspace of an 8-bit decode call on the current stream of device ``index``."""
+    global _q8_fixed_bytes
     L = _lib.lib()
+    if not _q8_fixed_bytes:
+        _q8_fixed_bytes = L.tvk_paged_decode_q8_workspace_size(0, 0)
     nbytes = L.tvk_paged_decode_q8_workspace_size(batch, n_kv_heads)
-    ws = _capture_workspace(device, nbytes, "decode_q8", nbytes - L.tvk_paged_decode_q8_workspace_size(0, 0))
-    return _workspace(device, nbytes, "decode_q8") if ws is None else ws
+    ws = _capture_workspace(index, nbytes, "decode_q8", nbytes - _q8_fixed_bytes)
+    if ws is None:
+        ws = _workspaces.get((index, _lib.raw_stream(index), "decode_q8"))
+        if ws is None or ws.numel() < nbytes:
+            ws = _workspace(torch.device("cuda", index), nbytes, "decode_q8")
+    return ws
 
 
 def workspace_status(device: Optional[torch.device] = None, kind: str = "decode") -> int:
@@ -80,7 +91,10 @@ def status_word(device: Optional[torch.device] = None, kind: str = "decode") -> 
     """The current stream's workspace status word as a one-element int32 device tensor
     (a view: a CUDA graph can copy it out alongside its results)."""
     device = device or torch.device("cuda", torch.cuda.current_device())
-    ws = _capture_workspace(device, 0, kind, 0) if kind == "decode_q8" else None
+    ws = None
+    if kind == "decode_q8":
+        index = device.index if device.index is not None else torch.cuda.current_device()
+        ws = _capture_workspace(index, 0, kind, 0)
     return (_workspace(device, 0, kind) if ws is None else ws)[:4].view(torch.int32)
 
 
@@ -160,24 +174,24 @@ def paged_decode_attention_q8(queries: torch.Tensor, k_cache: torch.Tensor, v_ca
     everything else, and the masking, as in ``paged_decode_attention``.  Returns
     [B,1,Hq,D] in the dtype of the queries.
     """
-    dev = _lib.require_cuda(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
-    B = queries.shape[0]
-    if queries.shape[1:] != (1, n_heads, head_dim):
-        raise ValueError(f"queries must be [B,1,{n_heads},{head_dim}], got {tuple(queries.shape)}")
-    if k_cache.dim() != 4 or k_cache.shape[1:] != (block_size, n_kv_heads, head_dim) or v_cache.shape != k_cache.shape:
+    dev = _lib.same_device(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+    qs, ks, ts = queries.shape, k_cache.shape, block_tables.shape
+    B = qs[0] if qs else 0
+    if qs[1:] != (1, n_heads, head_dim):
+        raise ValueError(f"queries must be [B,1,{n_heads},{head_dim}], got {tuple(qs)}")
+    if ks[1:] != (block_size, n_kv_heads, head_dim) or v_cache.shape != ks:
         raise ValueError(f"k_cache/v_cache must be [N,{block_size},{n_kv_heads},{head_dim}], got "
-                         f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
-    num_blocks = k_cache.shape[0]
+                         f"{tuple(ks)} / {tuple(v_cache.shape)}")
     if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise TypeError("k_cache and v_cache must be float8_e4m3fn")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError("k_scale and v_scale must be float32")
-    if k_scale.shape != (num_blocks, n_kv_heads) or v_scale.shape != k_scale.shape:
-        raise ValueError(f"k_scale/v_scale must be [{num_blocks},{n_kv_heads}], got {tuple(k_scale.shape)} / "
+    if k_scale.shape != (ks[0], n_kv_heads) or v_scale.shape != (ks[0], n_kv_heads):
+        raise ValueError(f"k_scale/v_scale must be [{ks[0]},{n_kv_heads}], got {tuple(k_scale.shape)} / "
                          f"{tuple(v_scale.shape)}")
     if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
         raise TypeError("block_tables and context_lens must be int32")
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or context_lens.shape != (B,):
+    if len(ts) != 2 or ts[0] != B or context_lens.shape != (B,):
         raise ValueError("block_tables must be [B,max_blocks] and context_lens [B]")
     if not (queries.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
             and k_scale.is_contiguous() and v_scale.is_contiguous() and block_tables.is_contiguous()
@@ -185,20 +199,19 @@ def paged_decode_attention_q8(queries: torch.Tensor, k_cache: torch.Tensor, v_ca
         raise ValueError("all tensors must be contiguous")
     if out is None:
         out = torch.empty_like(queries)
-    elif (out.shape != queries.shape or out.dtype != queries.dtype or out.device != dev
-          or not out.is_contiguous()):
+    elif (out.shape != qs or out.dtype != queries.dtype or out.get_device() != dev or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor like queries")
-    L = _lib.lib()
     ws = _workspace_q8(dev, B, n_kv_heads)
     rc = _lib.call_on(
-        dev, L.tvk_paged_decode_attention_q8, queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        dev, _lib.lib().tvk_paged_decode_attention_q8, queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-        B, n_heads, n_kv_heads, head_dim, block_size, num_blocks, block_tables.shape[1],
+        B, n_heads, n_kv_heads, head_dim, block_size, ks[0], ts[1],
         -1 if max_context_len is None else int(max_context_len), _lib.dtype_code(queries), ws.data_ptr(), ws.numel(),
-        _lib.stream_ptr(dev))
-    _lib.check(rc, "tvk_paged_decode_attention_q8")
+        _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "tvk_paged_decode_attention_q8")
     if check:
-        check_workspace(dev, "decode_q8", "tvk_paged_decode_attention_q8")
+        check_workspace(torch.device("cuda", dev), "decode_q8", "tvk_paged_decode_attention_q8")
     return out
 
 

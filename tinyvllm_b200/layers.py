@@ -145,14 +145,14 @@ def write_kv_slots_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     so the rows already there change their exponents only).  Rows with negative or
     out-of-pool slots are skipped; of several rows for one slot the last counts;
     values that are not finite are stored as NaN."""
-    dev = _lib.require_cuda(k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    _contig(k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError(f"k/v must be [T,Hkv,D] and the caches [N,block_size,Hkv,D], got {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    T, hkv, d = k.shape
-    nb, bs = k_cache.shape[:2]
-    if k_cache.shape[2:] != (hkv, d) or k_scale.shape != (nb, hkv) or v_scale.shape != (nb, hkv):
+    dev = _lib.same_device(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    shape, pool = k.shape, k_cache.shape
+    if len(shape) != 3 or v.shape != shape or len(pool) != 4 or v_cache.shape != pool:
+        raise ValueError(f"k/v must be [T,Hkv,D] and the caches [N,block_size,Hkv,D], got {tuple(shape)}, "
+                         f"{tuple(v.shape)}, {tuple(pool)}, {tuple(v_cache.shape)}")
+    T, hkv, d = shape
+    nb, bs = pool[0], pool[1]
+    if pool[2] != hkv or pool[3] != d or k_scale.shape != (nb, hkv) or v_scale.shape != (nb, hkv):
         raise ValueError(f"caches must be [N,block_size,{hkv},{d}] with scales [N,{hkv}]")
     if v.dtype != k.dtype:
         raise TypeError("k and v must share one dtype")
@@ -162,10 +162,14 @@ def write_kv_slots_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
         raise TypeError("k_scale and v_scale must be float32")
     if slots.dtype != torch.int64 or slots.shape != (T,):
         raise TypeError("slots must be int64 [T]")
+    if not (k.is_contiguous() and v.is_contiguous() and slots.is_contiguous() and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError("tensors must be contiguous")
     rc = _lib.call_on(dev, _lib.lib().tvk_write_kv_slots_q8, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
                       k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, hkv, d, nb, bs,
-                      _lib.dtype_code(k), _stream(dev))
-    _lib.check(rc, "tvk_write_kv_slots_q8")
+                      _lib.dtype_code(k), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "tvk_write_kv_slots_q8")
 
 
 def silu_mul(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -231,10 +235,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
 
     Equal logits rank in index order.  A token outside the vocabulary has -inf; a row
     with NaN or +inf, or with nothing but -inf, has NaN values."""
-    dev = _lib.require_cuda(logits, tokens)
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    dev = _lib.same_device(logits, tokens)
+    shape = logits.shape
+    if len(shape) != 2 or (logits.stride(1) != 1 and shape[1] > 1):
         raise ValueError("logits must be [R, V] with contiguous rows")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if not 0 <= top_k <= min(32, vocab):
         raise ValueError(f"top_k must be in [0, min(32, {vocab})], got {top_k}")
     if tokens.dtype != torch.int32 or tokens.shape != (rows,):
@@ -244,12 +249,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     row_stride = logits.stride(0) if rows > 1 else vocab
     if row_stride < vocab:
         raise ValueError("rows of logits must not overlap")
-    # one allocation for the three fp32 results, the tokens apart
-    f = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=dev)
-    lp, ent, top = f[:rows], f[rows:2 * rows], f[2 * rows:].view(rows, top_k)
-    top_tokens = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+    code = _lib.dtype_code(logits)
+    top_tokens = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device)
+    # one allocation for the three fp32 results
+    lp, ent, top = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=logits.device).split_with_sizes(
+        (rows, rows, rows * top_k))
+    top = top.view(rows, top_k)
     rc = _lib.call_on(dev, _lib.lib().tvk_token_logprobs, logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(),
-                      ent.data_ptr(), top.data_ptr(), top_tokens.data_ptr(), rows, vocab, row_stride, top_k,
-                      _lib.dtype_code(logits), _stream(dev))
-    _lib.check(rc, "tvk_token_logprobs")
+                      ent.data_ptr(), top.data_ptr(), top_tokens.data_ptr(), rows, vocab, row_stride, top_k, code,
+                      _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "tvk_token_logprobs")
     return TokenLogprobs(lp, ent, top, top_tokens)
