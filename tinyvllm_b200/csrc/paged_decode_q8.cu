@@ -1124,15 +1124,23 @@ int launch_tc(const Q8Params& p, cudaStream_t stream) {
 }
 
 // 16-bit queries on the tensor cores where 128-token tiles are whole blocks or lie in one.
-// Query heads per unit: as few as hold the group, but no more than 16 over the HP KV heads.
+// Query heads per unit (GP): as few as hold the group, but no more than 16 over the HP KV heads.
+// Calls that would leave most CTAs idle take units of 4 all the same: their tiles take half the
+// time, and the second reading of K and V comes from L2.  That is, of 4-head units either at
+// most 64 (32/4 heads of 64: one sequence of 512 tokens 12.9 -> 9.9 us, 8 of 8,192 22.5 -> 20.9),
+// or no more than there are CTAs, none of them cut (64 sequences of 40-640: 17.8 -> 15.5).
+// 32 sequences of 1,024 or 2,048 lose by it (17.4 -> 18.5, 20.6 -> 22.4).
 template <typename T>
 int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
   const int bs = p.block_size;
   if (!(bs == 8 || bs == 16 || bs == 32 || bs == 64 || bs % kTcTile == 0)) return launch_simt<T>(p, head_dim, stream);
   if (head_dim == 32) return launch_tc<T, 32, 4>(p, stream);
-  if (head_dim == 64) return p.group <= 4 ? launch_tc<T, 64, 4>(p, stream) : launch_tc<T, 64, 8>(p, stream);
-  return p.group <= 4 ? launch_tc<T, 128, 4>(p, stream)
-                      : p.group <= 8 ? launch_tc<T, 128, 8>(p, stream) : launch_tc<T, 128, 16>(p, stream);
+  const int pairs = head_dim == 64 ? (p.n_kv_heads + 1) / 2 : p.n_kv_heads;
+  const long long units = (long long)p.batch * pairs * ((p.group + 3) / 4);
+  const bool idle = units <= 64 || (units <= kTcCtas && tiles_of(p.max_ctx_tokens, kTcTile) <= kTcWhole);
+  if (head_dim == 64) return p.group <= 4 || idle ? launch_tc<T, 64, 4>(p, stream) : launch_tc<T, 64, 8>(p, stream);
+  if (p.group <= 4 || idle) return launch_tc<T, 128, 4>(p, stream);
+  return p.group <= 8 ? launch_tc<T, 128, 8>(p, stream) : launch_tc<T, 128, 16>(p, stream);
 }
 
 }  // namespace
