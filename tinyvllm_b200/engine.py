@@ -373,7 +373,11 @@ class LLMEngine:
                 if self._prefill_pool is None:
                     self._prefill_pool = torch.cuda.graph_pool_handle()
                     self._prefill_stream = torch.cuda.Stream(dev)
-                graph = self.model.capture_prefill(n, t_pad, self.kv_cache, self._prefill_pool, self._prefill_stream)
+                    # one for all prefill graphs: it is read before the next of them runs
+                    self._prefill_logits = torch.empty(self.max_batch_size, self.model.config.vocab_size,
+                                                       dtype=self.model.output.dtype, device=dev)
+                graph = self.model.capture_prefill(n, t_pad, self.kv_cache, self._prefill_pool, self._prefill_stream,
+                                                   self._prefill_logits)
                 self._prefill_graphs[(n, t_pad)] = graph
             sampled = graph.run(toks, pos, lens, slots).tolist()   # raises if a kernel wait timed out
             self._add_logprobs(graph.logits, graph.out[:n], seqs)

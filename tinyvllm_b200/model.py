@@ -233,13 +233,14 @@ class Llama:
 
     # ---------------------------------------------------------------- prefill
     def prefill(self, tokens: torch.Tensor, positions: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int,
-                slot_mapping: torch.Tensor, kv_cache: KVCache, n_out: Optional[int] = None) -> torch.Tensor:
+                slot_mapping: torch.Tensor, kv_cache: KVCache, n_out: Optional[int] = None,
+                logits_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Ragged prefill of several prompts packed along tokens.
 
         tokens/positions int32 [T]; cu_seqlens int32 [n+1]; slot_mapping int64 [T].
         Writes every layer's post-RoPE K and raw V into ``kv_cache`` at the slots
         (fused into the attention kernel) and returns the last-position logits
-        [n, vocab] (of the first ``n_out`` prompts only, when given).
+        [n, vocab] (of the first ``n_out`` prompts only, when given; in ``logits_out``, when given).
         """
         c = self.config
         T = tokens.shape[0]
@@ -256,13 +257,16 @@ class Llama:
             nxt = self.layers[i + 1].attention_norm if i + 1 < c.n_layers else self.norm
             x = self._layer_ffn(L, h, attn, nxt, T)
         last = (cu_seqlens[1:] if n_out is None else cu_seqlens[1:n_out + 1]) - 1
-        return torch.matmul(x[last.long()], self.output)
+        return torch.matmul(x[last.long()], self.output, out=logits_out)
 
     def capture_prefill(self, n_prompts: int, padded_tokens: int, kv_cache: "KVCache",
-                        pool=None, stream: Optional[torch.cuda.Stream] = None) -> "PrefillGraph":
+                        pool=None, stream: Optional[torch.cuda.Stream] = None,
+                        logits: Optional[torch.Tensor] = None) -> "PrefillGraph":
         """A CUDA graph of one ragged prefill of ``n_prompts`` prompts totalling fewer
-        than ``padded_tokens`` tokens, plus the greedy pick of each prompt's first token."""
-        return PrefillGraph(self, n_prompts, padded_tokens, kv_cache, pool, stream)
+        than ``padded_tokens`` tokens, plus the greedy pick of each prompt's first token.
+        ``logits`` [>= n_prompts, vocab] is where its logits go: graphs that replay one
+        after the other may share it."""
+        return PrefillGraph(self, n_prompts, padded_tokens, kv_cache, pool, stream, logits)
 
     def capture_decode(self, batch: int, table_width: int, kv_cache: "KVCache",
                        kv_order: str = "reference") -> "DecodeGraph":
@@ -350,7 +354,7 @@ class DecodeGraph:
 
     def _forward(self):
         logits = self.model.decode(self.tok, self.pos, self.bt, self.ctx, self.slots, self.kv_cache, self.kv_order)
-        self.logits = logits    # of the last replay; its rows stay until the next one
+        self.logits = logits    # of the last replay, until the next one
         layers.greedy_argmax(logits, out=self.out[:self.batch])
         # the attention calls of this step used this stream's workspace; the view
         # also keeps that workspace alive for as long as the graph exists
@@ -433,7 +437,7 @@ class PrefillGraph:
     """
 
     def __init__(self, model: Llama, n: int, T: int, kv_cache: KVCache, pool=None,
-                 stream: Optional[torch.cuda.Stream] = None):
+                 stream: Optional[torch.cuda.Stream] = None, logits: Optional[torch.Tensor] = None):
         if n < 1 or T < n + 1:
             raise ValueError("a prefill graph needs n >= 1 prompts and T > n tokens")
         dev = model.device
@@ -447,6 +451,9 @@ class PrefillGraph:
         self.slots = self.d_in[self._off_slots:].view(torch.int64)
         self.out = torch.zeros(n + 1, dtype=torch.int32, device=dev)   # tokens, then the status word
         self.h_out = torch.zeros(n + 1, dtype=torch.int32).pin_memory()
+        if logits is None:
+            logits = torch.empty(n, model.config.vocab_size, dtype=model.output.dtype, device=dev)
+        self.logits = logits[:n]    # of the last replay
         self._stage(np.zeros(0, np.int32), np.zeros(0, np.int32), None, np.zeros(0, np.int64))
         self.d_in.copy_(self.h_in)
         self.stream = stream or torch.cuda.Stream(dev)
@@ -462,8 +469,8 @@ class PrefillGraph:
 
     def _forward(self):
         m = self.model
-        logits = m.prefill(self.tok, self.pos, self.cu, self.T, self.slots, self.kv_cache, n_out=self.n)
-        self.logits = logits    # of the last replay; its rows stay until the next one
+        logits = m.prefill(self.tok, self.pos, self.cu, self.T, self.slots, self.kv_cache, n_out=self.n,
+                           logits_out=self.logits)
         layers.greedy_argmax(logits, out=self.out[:self.n])
         # the attention calls used this stream's prefill workspace; the view keeps it
         # alive for as long as the graph exists
