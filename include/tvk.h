@@ -294,7 +294,8 @@ size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads);
  *   K_t = k_scale[blk, h/g] * k_cache[blk, off, h/g], V_t likewise.
  * q and out are fp32, fp16 or bf16; head_dim 32, 64 or 128; at most 16 query heads
  * per KV head; any block size.  What lies behind a sequence's context is never
- * used, whatever it holds.  q, k_cache and v_cache 16-byte aligned.
+ * used, whatever it holds.  Scales are zero or positive; a block whose v_scale is negative
+ * gives NaN.  q, k_cache, v_cache and workspace 16-byte aligned, out 4-byte; out does not overlap q.
  */
 int tvk_paged_decode_attention_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                   const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,
@@ -358,10 +359,10 @@ int tvk_paged_decode_noalloc_status(int* status, void* stream);
 
 /*
  * Test hook for the kernels' bounded waits (no counterpart in the reference).
- * Arms the next tvk_paged_decode_attention / tvk_flash_prefill_attention call
- * made on the calling thread that reaches a tensor-core kernel (fp16/bf16):
+ * Arms the next tvk_paged_decode_attention, tvk_paged_decode_attention_q8 or
+ * tvk_flash_prefill_attention call made on the calling thread that reaches a tensor-core kernel (fp16/bf16):
  * that launch gets `limit_ns` (1e5 .. 2e9) as the wall-time limit of its
- * mbarrier waits, and its producer warp issues no loads, so the consumers'
+ * mbarrier waits, and its producer warps issue no loads, so the consumers'
  * first wait runs out.  The kernel then sets the workspace status word to 1
  * and returns; nothing faults, traps or hangs.  The caller must zero the
  * workspace header (256 bytes) before the next call.  One-shot: the arming is

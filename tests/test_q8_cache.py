@@ -318,6 +318,11 @@ def test_python_refusals(cuda):
             _run({**c, name: bad})
     with pytest.raises(ValueError):
         _run(c, out=torch.empty(2, 1, 8, 64, device=cuda))
+    room = torch.zeros(2 * c["q"].numel(), dtype=c["q"].dtype, device=cuda)
+    q = room[:c["q"].numel()].view(c["q"].shape)
+    for off in (0, 8, c["q"].numel() - 8):
+        with pytest.raises(TvkError, match="overlap"):
+            _run({**c, "q": q}, out=room[off:off + q.numel()].view(q.shape))
     x, codes, scale, slots = _write_case(cuda, 4, 2, 64, 16, 8, torch.float16, 6, lambda rng: [0, 1, 2, 3])
     good = [*x, slots, *codes, *scale]
     for i, bad, err in ((0, x[0].double(), TypeError), (2, slots.int(), TypeError), (2, slots[:3], TypeError), (3, codes[0].float(), TypeError),
@@ -376,6 +381,41 @@ def test_two_graphs_recorded_on_one_stream_replay_at_once(cuda):
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_branches_of_one_graph_and_many_recordings(cuda):
+    """Two branches of a graph that may run at once each have a workspace, and recordings of graphs that are dropped leave no memory behind."""
+    cs = [_case(cuda, 3, 32, 8, 128, 16, ctx, torch.float16, s) for s, ctx in ((1, [5000, 700, 9000]), (2, [8000, 0, 3000]))]
+    want = [_run(c).clone() for c in cs]
+    outs = [torch.empty_like(w) for w in want]
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def record():
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=main):
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                for _ in range(4):
+                    _run(cs[1], out=outs[1])
+            for _ in range(4):
+                _run(cs[0], out=outs[0])
+            main.wait_stream(side)
+        return g
+
+    g = record()
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    held = []
+    for _ in range(6):
+        del g
+        g = record()
+        torch.cuda.synchronize()
+        held.append(torch.cuda.memory_allocated())
+    assert held[-1] == held[1]
 
 
 def test_wait_that_runs_out_is_told_and_the_next_call_is_right(cuda):

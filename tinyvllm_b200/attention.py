@@ -34,14 +34,15 @@ def _workspace(device: torch.device, nbytes: int, kind: str = "decode") -> torch
         return ws
 
 
-_capture_workspaces: Dict[tuple, torch.Tensor] = {}
+_capture_workspaces: Dict[tuple, Tuple[int, torch.Tensor]] = {}
 
 
 def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Optional[torch.Tensor]:
-    """While the current stream records a CUDA graph: a workspace of that graph alone, so that
-    graphs recorded on one stream may run at the same time.  Its header and last
-    ``zero_tail`` bytes are zeroed by the graph itself at every replay.  It lives as long
-    as the process, as the per-stream workspaces do.  None while nothing is recorded."""
+    """While the current stream records a CUDA graph: a workspace of that graph and stream
+    alone, so that graphs recorded on one stream, and branches of one graph, may run at
+    the same time.  Its header and last ``zero_tail`` bytes are zeroed by the graph itself
+    at every replay.  It lies in the graph's memory pool and lives as long as that; here
+    it is only kept until the stream's next recording.  None while nothing is recorded."""
     if not torch.cuda.is_current_stream_capturing():
         return None
     capture = ctypes.c_ulonglong()
@@ -49,16 +50,15 @@ def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Op
     _lib.check(rc, "tvk_stream_capture_id")
     if capture.value == 0:               # another device's stream is the one that records
         return None
-    key = (index, capture.value, kind)
+    key = (index, _lib.raw_stream(index), kind)
     with _ws_lock:
-        ws = _capture_workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
+        of, ws = _capture_workspaces.get(key, (0, None))
+        if of != capture.value or ws.numel() < nbytes:
+            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", index))
             ws[:256].zero_()
             if zero_tail:
-                ws[ws.numel() - zero_tail:].zero_()
-            _capture_workspaces[(*key, ws.data_ptr())] = ws     # what a replay uses is never freed
-            _capture_workspaces[key] = ws
+                ws[nbytes - zero_tail:].zero_()
+            _capture_workspaces[key] = (capture.value, ws)
         return ws
 
 

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const Wri
     }
     __syncthreads();
     auto look = [&](long long slot, int i) {
-      const unsigned long long d = (unsigned long long)(slot - base);
+      const unsigned long long d = (unsigned long long)slot - (unsigned long long)base;
       if (d < (unsigned long long)bs) {
         atomicMax(&row_of[d], i);
         if (i < t) atomicMin(&first, i);

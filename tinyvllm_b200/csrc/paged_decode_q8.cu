@@ -38,7 +38,7 @@ constexpr int kTcCtas = 296;         // two CTAs on each SM
 constexpr int kMaxPieces = kSimtCtas;
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
 constexpr int kMaxParts = 4;         // units per (sequence, KV head) at most, where groups are split
-constexpr int kSlotFloats = 2240;    // partials of one cut unit: rows * (D + 2), at most 64 * 34, 32 * 66 or 16 * 130
+constexpr int kSlotFloats = 2080;    // partials of one cut unit: rows * (D + 2), at most 16 * 130
 
 struct Q8Params {
   const void* q;
@@ -371,9 +371,15 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
 //    p1 + p2 + 2^-8 p3: exact down to 2^-18, where the largest counts as 2^4..2^8.
 // The matrix unit sums in fp32.  So nothing is converted per K/V element: the work of
 // the CUDA cores is per (token, query head).  (Decoding the codes to halves for
-// mma.sync took 470 instructions per 16 tokens and 265 us where this takes 218 us:
-// 256 sequences of 128-4096 tokens, 32/8 heads of 128.  mma.sync on e4m3 itself
-// is converted to halves by the compiler on this architecture and took longer still.)
+// mma.sync took 470 instructions per 16 tokens and 265 us where this took 218 us in
+// its first form: 256 sequences of 128-4096 tokens, 32/8 heads of 128.  mma.sync on e4m3
+// itself is emulated on this architecture and took longer still.)
+//
+// Now that call takes 184-198 us (from box to box), 5.7-6.1 TB/s of codes and scales, 0.87-0.92
+// of the measured copy rate: memory bounds units of 4 heads.  With 8 heads a unit
+// 5.5 TB/s, with 16 2.9 TB/s (32/4 and 32/2 heads of 128, the same sequences):
+// there the softmax warps' work per (token, query head) bounds it, about half of that
+// the three parts of a weight and their byte stores.
 //
 // Roles: warp 0 streams K tiles (TMA) and their scales (4-byte asynchronous
 // copies), warp 3 V; warp 1 issues the products; warp 2 splits the query rows of the next share;
@@ -386,7 +392,10 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
 // They move only when a weight would pass 2^8 (or a sum's term 2^64); then O^T is rescaled.
 // -----------------------------------------------------------------------------
 constexpr int kTcThreads = 256;
-constexpr int kScaleRing = 8;  // tiles whose scales are kept: a K slot comes round only when S^T of 5 tiles later is read
+// Tiles whose scales are kept.  A producer writes a tile's scales once it has the tile's slot, which is free when
+// the product of the tile at least (kSlots - 1) / 2 before is done; S^T being double, the softmax is at most two
+// tiles behind that: 7 slots make 5 tiles in all.
+constexpr int kScaleRing = 8;
 constexpr float kLowPart = 0.00390625f;
 
 template <int D, int GP>
@@ -412,7 +421,8 @@ struct TcLayout {
   static constexpr int kBarOff = kMiscOff + kMisc;
   static constexpr int kBytes = kBarOff + kBars + 1024;
   static_assert(HG <= 16 && kOCol + NO <= 256 && kSlots >= 5 && kSlots <= 7, "sizes");
-  static_assert((2 * kSlots + kScaleRing + 14) * 8 <= kBars, "barriers");
+  static_assert((2 * kSlots + kScaleRing + 15) * 8 <= kBars, "barriers");
+  static_assert(HG * (D + 2) <= kSlotFloats, "partials");
   static_assert(2 * kP / 4 >= HG * 8, "room for the join's factors of some parts at a time");
 };
 
@@ -488,7 +498,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   uint64_t* q_full = p_empty + 2;            // [QB] query parts written
   uint64_t* q_empty = q_full + 2;            // [QB] the share's S^T all done, query factors read
   uint64_t* o_empty = q_empty + 2;           // O^T read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
+  uint64_t* drain = o_empty + 1;             // after a wait that ran out: every product issued is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   // misc: per head {limit of s + log2 v_scale, limit of s, M, R}, query factors [2][16], warp results
   // [4][16][2], two factors per head [16][2], a flag
   float4* ref_s = reinterpret_cast<float4*>(base + L::kMiscOff);
@@ -514,6 +525,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       ptx::mbar_init(&q_empty[i], 5);
     }
     ptx::mbar_init(o_empty, 4);
+    ptx::mbar_init(drain, 1);
     ptx::fence_mbar_init();
   }
   if (warp == 1) {
@@ -629,6 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
     // No copy is in flight when the CTA ends, whatever became of the others.
     const uint32_t total = 2 * it;
+    // (After a wait that ran out the last copy was issued before it, a whole limit ago.)
     for (uint32_t n = total > SL ? total - SL : 0; n < total && ok && !p.drop_loads; ++n)
       if ((n == total - 1 || (n > 0 && n % 2 == 0)) == is_v) ok = warp_wait(&full_bar[slot_of(n)], round_of(n), p.wait_ns);
   } else if (warp == 1) {
@@ -711,7 +724,14 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (ok) issue_pv();
       ok = ok && warp_wait(&p_empty[due_tile & 1], (due_tile >> 1) & 1, p.wait_ns);  // nothing runs when TMEM is freed
     }
-    if (!ok && lane == 0) atomicExch(p.status, tvk::kStatusWaitTimeout);
+    if (!ok) {
+      if (lane == 0) {
+        atomicExch(p.status, tvk::kStatusWaitTimeout);
+        umma::commit(drain);
+      }
+      __syncwarp();
+      warp_wait(drain, 0, p.wait_ns);
+    }
   } else if (warp == 2) {
     // ---------------- query rows of each share, in parts ----------------
     constexpr int LPR = D / 4;     // lanes per row, four elements each
@@ -1176,7 +1196,11 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
                 "null pointer argument");
   TVK_CHECK_ARG(((uintptr_t)q % 16 == 0) && ((uintptr_t)k_cache % 16 == 0) && ((uintptr_t)v_cache % 16 == 0) &&
                     ((uintptr_t)out % 4 == 0),
-                "q, k_cache and v_cache must be 16-byte aligned");
+                "q, k_cache and v_cache must be 16-byte aligned, out 4-byte");
+  // a query row is read by every CTA that shares its sequence, whoever has written its output by then
+  const uintptr_t q0 = (uintptr_t)q, o0 = (uintptr_t)out;
+  const uintptr_t extent = (uintptr_t)batch * n_heads * head_dim * tvk::dtype_size(dtype);
+  TVK_CHECK_ARG(q0 + extent <= o0 || o0 + extent <= q0, "out must not overlap q");
   const size_t need = tvk_paged_decode_q8_workspace_size(batch, n_kv_heads);
   if (!workspace || workspace_bytes < need) {
     tvk::set_error("workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
