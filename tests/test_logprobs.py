@@ -121,6 +121,29 @@ def test_peaked_and_flat_rows(cuda, dtype):
         _check(*_logits(cuda, 4, 32000, dtype, 9, spread), 20)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [20000, 150001, 300004])
+def test_long_rows_of_many(cuda, dtype, V):
+    """More rows than share a GPU by clusters, each a CTA's with many steps: six kinds of rows among 260."""
+    from tinyvllm_b200 import layers
+    rng = np.random.default_rng(V)
+    x = rng.normal(size=(6, V)) * 4
+    x[1] = np.sort(x[1])                          # every step beats the ones before: the buffer runs over
+    x[2] = np.sort(x[2])[::-1]
+    x[3] = 1.5
+    x[4, rng.random(V) < 0.9] = -np.inf
+    x[5, :V - 40] = -np.inf
+    at = np.asarray([0, 51, 103, 148, 200, 259])
+    few = torch.from_numpy(x).to(dtype).to(cuda)
+    logits = torch.randn(260, V, device=cuda, dtype=torch.float32).to(dtype)
+    logits[torch.from_numpy(at).to(cuda)] = few
+    tok = torch.from_numpy(rng.integers(0, V, 260).astype(np.int32)).to(cuda)
+    for k in (0, 1, 5, 32):
+        got = layers.token_logprobs(logits, tok, k)
+        idx = torch.from_numpy(at).to(cuda)
+        _check(few, tok[idx], k, layers.TokenLogprobs(*(t[idx] for t in got)))
+
+
 def test_agrees_with_greedy_argmax(cuda):
     from tinyvllm_b200 import layers
     x, tok = _logits(cuda, 64, 32000, torch.float16, 4)

@@ -7,36 +7,46 @@
 //                with S = sum exp(x_v - m), T = sum exp(x_v - m) (x_v - m)
 //   top[r]     = the K largest logits, equal values in index order
 //
-// Each thread keeps (m, S, T) in fp32 for the logits it reads, 16 bytes at a
-// time; its m moves only when a vector exceeds it by more than 4 (moving at every new
+// Each thread keeps (m, S, T) in fp32 for the logits it reads, four 16-byte vectors a
+// step; its m moves only when a step exceeds it by more than 4 (moving at every new
 // maximum, some lane of a warp did so in most steps, which cost a third of the time).
 //
-// The K best: from the maxima of 32 groups of threads over the first step (4
-// vectors a thread) each CTA takes the K-th largest as a threshold, which K
-// logits at least reach; one below it is not among the K best.  What reaches it is
-// pushed as a 64-bit key (ordered value, inverted index) to shared memory; the same
-// with groups of keys raises the threshold once more after a few steps, and leaves little
-// more than the K best for ranking at the end.
+// A row to itself (many rows) is a CTA's, whose vectors travel through shared memory a
+// step ahead: [2048, 128256] bf16 with one alternative takes 100 us so (5.2 TB/s, 0.80 of
+// the measured copy rate), with loads to registers 145 us, when a warp had nothing in flight
+// while it computed (and loads a step ahead in registers 203 us).  Without alternatives
+// 88 us; fp32 logits 157 and 162 us, 6.7 TB/s, all that memory gives.  What is left for bf16
+// is the exponentials (58 us of the special-function unit) and the candidates' barriers.
+// With few rows a cluster of CTAs shares each, and their sums and K best are put
+// together by the first over distributed shared memory; they read once and are done, so
+// latencies bound them ([1, 128256] bf16 7.0 us, [64, 32000] fp16 with 20 alternatives 8.9 us).
+//
+// The K best: from the maxima of 64 groups of threads over the first step
+// each CTA takes the K-th largest as a threshold, which K logits at least reach; one
+// below it is not among the K best.  What reaches it is pushed as a 64-bit key (ordered
+// value, inverted index) to shared memory; the same with groups of keys raises the threshold
+// after 4, 8 and 16 steps and every 16 from there, and leaves little more than the K best for
+// ranking at the end.  [2048, 128256] bf16 takes 127 us with K = 8, 157 with 20, 185 with 32
+// (with 32 groups and one raise 123, 183 and 429): pushing is what it costs.
 // Rows that keep pushing (sorted or constant logits) run into the buffer's
 // limit, are cut back to their K best and go on with an exact threshold.
-//
-// With few rows a cluster of CTAs shares each: the CTAs' sums and K best are put
-// together by the first over distributed shared memory.
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "tvk_common.cuh"
 
 namespace {
 
-constexpr int kLpUnroll = 4;         // 16-byte loads in flight per thread
-constexpr int kLpSteps = 4;          // steps between two looks at the candidate buffer
+constexpr int kLpUnroll = 4;         // 16-byte vectors a thread reads per step
+constexpr int kLpFirstSteps = 4, kLpSteps = 16;  // steps before the first look at the candidate buffer, and between two
 constexpr float kLpSlack = 4.f;      // a reference may lie this far below its thread's largest logit
 constexpr int kLpBuf = 2048;         // candidate keys kept in shared memory
 constexpr int kLpMaxK = 32;
+constexpr int kLpGroups = 64;        // groups of threads, or of keys, whose maxima give a threshold
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLpFloor = -30000.f;  // see add_vec
+constexpr float kLpFloor = -30000.f;  // see add_step
 
 // fp32 values as unsigned integers of the same order: -0 counts as +0, every
 // NaN as one value above +inf.
@@ -55,20 +65,37 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// The larger of all elements of one 16-byte vector, NaN if one is.
-template <typename T> __device__ __forceinline__ float vec_max(const uint4& u);
-template <> __device__ __forceinline__ float vec_max<float>(const uint4& u) {
-  return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+// The larger elements of two 16-byte vectors, NaN where one is.
+template <typename T> __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
+  uint4 r;
+  const uint32_t *x = &a.x, *y = &b.x;
+  uint32_t* z = &r.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      z[i] = __float_as_uint(max_nan(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2 m = __hmax2_nan(*reinterpret_cast<const T2*>(&x[i]), *reinterpret_cast<const T2*>(&y[i]));
+      z[i] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  return r;
 }
-template <> __device__ __forceinline__ float vec_max<__half>(const uint4& u) {
-  const __half2* h = reinterpret_cast<const __half2*>(&u);
-  const __half2 c = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-  return __half2float(__hmax_nan(c.x, c.y));
+// The largest element of one vector, NaN if one is.
+template <typename T> __device__ __forceinline__ float vec_max(const uint4& u) {
+  const uint4 v = larger<T>(u, make_uint4(u.z, u.w, u.z, u.w));
+  if constexpr (sizeof(T) == 4) {
+    return max_nan(__uint_as_float(v.x), __uint_as_float(v.y));
+  } else {
+    const uint4 w = larger<T>(v, make_uint4(v.y, v.y, v.y, v.y));
+    const uint16_t lo = (uint16_t)w.x, hi = (uint16_t)(w.x >> 16);
+    return DT<T>::to_f(__hmax_nan(*reinterpret_cast<const T*>(&lo), *reinterpret_cast<const T*>(&hi)));
+  }
 }
-template <> __device__ __forceinline__ float vec_max<__nv_bfloat16>(const uint4& u) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-  const __nv_bfloat162 c = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-  return __bfloat162float(__hmax_nan(c.x, c.y));
+// Four bytes of -inf.
+template <typename T> __device__ __forceinline__ uint32_t minus_inf() {
+  return sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 }
 
 // Element e of a vector, without a register array.
@@ -201,25 +228,34 @@ __device__ __forceinline__ void add_pair(Sums& a, F2 x) {
   a.t = fma2(e, u, a.t);
 }
 
-// A whole vector.  With an ordinary reference (almost always) 16-bit elements are floored two
+// A step's vectors.  With an ordinary reference (almost always) 16-bit elements are floored two
 // at a time: what lies below -30000 weighs nothing beside it, and no product with -inf arises.
-template <typename T>
-__device__ __forceinline__ void add_vec(Sums& a, const uint4& u) {
+// The first n vectors; ALL: every one, without a branch between them.
+template <typename T, bool ALL>
+__device__ __forceinline__ void add_step(Sums& a, const uint4 (&u)[kLpUnroll], int n) {
   constexpr int N = 16 / sizeof(T);
   if (sizeof(T) == 2 && a.m > kLpFloor + 1000.f && a.m < INFINITY) {
-    const uint4 w = floored<T>(u);
     const F2 scale = pack(kLog2e, kLog2e), minus_m = pack(-a.m, -a.m);
 #pragma unroll
-    for (int e = 0; e < N / 2; ++e) {
-      const F2 y = mul2(add2(pair_of<T>(w, e), minus_m), scale);
-      const float2 v = unpack(y);
-      const F2 z = pack(ptx::ex2(v.x), ptx::ex2(v.y));
-      a.s = add2(a.s, z);
-      a.t = fma2(z, y, a.t);
+    for (int k = 0; k < kLpUnroll; ++k) {
+      if (!ALL && k >= n) break;
+      const uint4 w = floored<T>(u[k]);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const F2 y = mul2(add2(pair_of<T>(w, e), minus_m), scale);
+        const float2 v = unpack(y);
+        const F2 z = pack(ptx::ex2(v.x), ptx::ex2(v.y));
+        a.s = add2(a.s, z);
+        a.t = fma2(z, y, a.t);
+      }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < N / 2; ++e) add_pair(a, pair_of<T>(u, e));
+    for (int k = 0; k < kLpUnroll; ++k) {
+      if (!ALL && k >= n) break;
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) add_pair(a, pair_of<T>(u[k], e));
+    }
   }
 }
 
@@ -246,8 +282,10 @@ struct LpParams {
 };
 
 // NT: threads of a CTA.  A row to itself gets 256 (four CTAs on an SM: a row's serial end hides
-// behind three others' loads), a cluster's share 512.  [2048, 128256] bf16 takes 145 us with 256 and 152 with 512,
-// one row of it on 8 CTAs 8.4 and 7.4, 37 x 50,001 fp32 on 4 CTAs each 10.5 and 9.3.
+// behind three others' loads), a cluster's share 512, read straight to registers: each thread has two
+// steps or so, so there is nothing to run ahead of.  With loads to registers [2048, 128256] bf16 took 145 us with 256 and
+// 152 with 512, one row of it on 8 CTAs 8.4 and 7.4, 37 x 50,001 fp32 on 4 CTAs each 10.5 and 9.3; those
+// 37 rows took 9.8 through shared memory.
 template <int NT>
 struct LpShared {
   unsigned long long keys[kLpBuf];
@@ -255,7 +293,8 @@ struct LpShared {
   RowSums sums;                      // and its part of the row's sums
   RowSums all_sums[8];
   float part[NT / 32][2];
-  uint32_t group_max[32], at_k;
+  alignas(16) uint32_t group_max[kLpGroups];
+  uint32_t at_k;
   int count, n_best;
   int wsum[NT / 32];
 };
@@ -326,6 +365,13 @@ __device__ __forceinline__ unsigned long long key_of(float x, int idx) {
   return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - (uint32_t)idx);
 }
 
+// Asynchronous 16-byte copy global -> shared, and the thread's wait for all groups of copies but the newest.
+__device__ __forceinline__ void copy16_async(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_copies_but_1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
@@ -361,29 +407,35 @@ __device__ __forceinline__ float block_max(LpShared<NT>& sh, float x) {
 template <int NT>
 __device__ __forceinline__ uint32_t kth_of_groups(LpShared<NT>& sh, int K) {
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    const uint32_t mine = sh.group_max[lane];
-    int above = 0;
+  if (K == 1) {  // every warp for itself
+    const uint32_t* g = sh.group_max + (threadIdx.x & 31);
+    static_assert(kLpGroups == 64, "two a lane");
+    return __reduce_max_sync(0xffffffffu, max(g[0], g[32]));
+  }
+  if (threadIdx.x < kLpGroups) {  // a warp or two
+    const uint32_t mine = sh.group_max[threadIdx.x];
+    int above = 0, not_below = 0;  // mine is the K-th largest where above < K <= not_below
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
-      above += other > mine || (other == mine && j < lane);
+    for (int j = 0; j < kLpGroups; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&sh.group_max[j]);
+      above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+      not_below += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
     }
-    if (above == K - 1) sh.at_k = mine;
+    if (above < K && K <= not_below) sh.at_k = mine;  // the same value, where several have it
   }
   __syncthreads();
   return sh.at_k;
 }
 
-// A value that K keys of the buffer at least reach (0: none found), by groups of keys.
+// A value that K keys of the buffer at least reach (0: none found), by groups of keys.  Between a barrier
+// before it and its own last one nothing is pushed.
 template <int NT>
 __device__ uint32_t reached_by_k(LpShared<NT>& sh, int K) {
   const int tid = threadIdx.x;
-  if (tid < 32) sh.group_max[tid] = 0u;
+  if (tid < kLpGroups) sh.group_max[tid] = 0u;
   __syncthreads();
   const int n = min(sh.count, kLpBuf);
-  for (int i = tid; i < n; i += NT) atomicMax(&sh.group_max[i & 31], (uint32_t)(sh.keys[i] >> 32));
+  for (int i = tid; i < n; i += NT) atomicMax(&sh.group_max[i % kLpGroups], (uint32_t)(sh.keys[i] >> 32));
   return kth_of_groups(sh, K);
 }
 
@@ -430,16 +482,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
   const uint32_t ctas = cluster_size(), rank = blockIdx.x % ctas;
   const long long row = blockIdx.x / ctas;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.row_stride;
-  float x_tok = 0.f;
-  bool inside = false;  // a token outside the vocabulary has probability 0
-  if (tid == 0) {
-    sh.count = 0;
-    if (rank == 0) {
-      const int tok = p.tokens[row];
-      inside = tok >= 0 && tok < V;
-      if (inside) x_tok = DT<T>::to_f(x[tok]);
-    }
-  }
+  if (tid == 0) sh.count = 0;
   // Elements before the first 16-byte boundary and after the last whole vector go one to a thread.
   const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
   const int all_vec = (V - head) / N, tail0 = head + all_vec * N;
@@ -448,6 +491,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
   Sums a{-INFINITY, pack(0.f, 0.f), pack(0.f, 0.f)};
   unsigned long long tau_key = 0ull;  // only keys above it are candidates
   float tau = -INFINITY;              // only values not below it are
+  // Each thread's vectors of a step travel to places of its own in shared memory while it works on those of
+  // the step before: no other thread reads them, so no barrier is needed, and no register waits for them.
+  constexpr bool kRing = NT == 256;
+  extern __shared__ uint4 ring[];  // [2][kLpUnroll][NT]
+  auto fetch = [&](int half, int base) {
+#pragma unroll
+    for (int k = 0; k < kLpUnroll; ++k) {
+      const int i = base + k * NT + tid;
+      if (i < v1) copy16_async(ring + (half * kLpUnroll + k) * NT + tid, xv + (size_t)i * N);
+    }
+    commit_copies();
+  };
+  int half = 0;
+  if constexpr (kRing) fetch(0, v0);
+  // The row's token and its logit, wanted at the end only: asked for behind the first vectors.
+  int tok = -1;
+  if (tid == 0 && rank == 0) tok = p.tokens[row];
   __syncthreads();
 
   auto push = [&](float f, int idx) -> bool {  // true: the buffer is getting full
@@ -458,6 +518,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
     return at >= kLpBuf / 2;
   };
 
+  const bool inside = tok >= 0 && tok < V;  // a token outside the vocabulary has probability 0
+  const float x_tok = inside ? DT<T>::to_f(x[tok]) : 0.f;
   if (rank == 0) {
     const int single = tid < head ? tid : (tid < head + V - tail0 ? tail0 + tid - head : -1);
     if (single >= 0) {
@@ -468,40 +530,48 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
     }
   }
 
-  for (int from = v0; from < v1; from += kLpSteps * kLpUnroll * NT) {
-    const int to = min(from + kLpSteps * kLpUnroll * NT, v1);
+  constexpr int kFirst = kLpFirstSteps * kLpUnroll * NT, kMost = kLpSteps * kLpUnroll * NT;
+  for (int from = v0, to; from < v1; from = to) {
+    to = min(from + min(max(kFirst, from - v0), kMost), v1);  // after 4, 8, 16 and every 16 further steps
     bool full = false;
     for (int base = from; base < to; base += kLpUnroll * NT) {
-      uint4 u[kLpUnroll];
-      float vm[kLpUnroll];
+      uint4 u[kLpUnroll];  // -inf where there is no vector
+      if constexpr (kRing) {
+        fetch(half ^ 1, base + kLpUnroll * NT);  // into the places read in the step before
+        wait_for_copies_but_1();
+      }
 #pragma unroll
       for (int k = 0; k < kLpUnroll; ++k) {
         const int i = base + k * NT + tid;
-        if (i < to) u[k] = __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
+        u[k] = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
+        if (i < to) u[k] = kRing ? ring[(half * kLpUnroll + k) * NT + tid] : __ldcs(reinterpret_cast<const uint4*>(xv + (size_t)i * N));
       }
-      float tm = -INFINITY;
+      half ^= 1;
+      uint4 all = larger<T>(u[0], u[1]);
 #pragma unroll
-      for (int k = 0; k < kLpUnroll; ++k) {
-        if (base + k * NT + tid < to) {
-          vm[k] = vec_max<T>(u[k]);
-          tm = max_nan(tm, vm[k]);
-          if (!(vm[k] <= a.m + kLpSlack)) raise_max(a, vm[k]);
-          add_vec<T>(a, u[k]);
-        }
-      }
+      for (int k = 2; k < kLpUnroll; ++k) all = larger<T>(all, u[k]);
+      const float tm = vec_max<T>(all);
+      if (!(tm <= a.m + kLpSlack)) raise_max(a, tm);
+      if (base + kLpUnroll * NT <= to)
+        add_step<T, true>(a, u, kLpUnroll);
+      else
+        add_step<T, false>(a, u, (to - base + NT - 1) / NT);
       if (K == 0) continue;
       if (base == v0) {
-        // The K-th largest of the maxima of 32 groups of threads: K logits at least are not below it.
+        // The K-th largest of the maxima of the groups of threads: K logits at least are not below it.
         const uint32_t o = tid < v1 - v0 ? order_of(tm) : 0u;
-        const uint32_t top = __reduce_max_sync(NT == 512 ? 0xffffu << (lane & 16) : 0xffu << (lane & 24), o);
-        if (tid % (NT / 32) == 0) sh.group_max[tid / (NT / 32)] = top;
+        uint32_t top = o;
+#pragma unroll
+        for (int d = 1; d < NT / kLpGroups; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (tid % (NT / kLpGroups) == 0) sh.group_max[tid / (NT / kLpGroups)] = top;
         const uint32_t at_k = kth_of_groups(sh, K);
         if (at_k) tau = value_of(at_k);  // 0: fewer than K groups have elements
       }
+      if (tm < tau) continue;
 #pragma unroll
       for (int k = 0; k < kLpUnroll; ++k) {
         const int i = base + k * NT + tid;
-        if (i < to && !(vm[k] < tau)) {
+        if (i < to && !(vec_max<T>(u[k]) < tau)) {
           for (uint32_t bits = not_below<T>(u[k], tau); bits; bits &= bits - 1) {
             const int e = __ffs(bits) - 1;
             full |= push(DT<T>::to_f(element<T>(u[k], e)), head + i * N + e);
@@ -511,10 +581,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
     }
     if (K == 0) continue;
     if (!__syncthreads_or(full)) {
-      if (from == v0 && to < v1 && sh.count > 2 * K) {
-        const uint32_t least = reached_by_k(sh, K);
+      if (to < v1) {
+        const bool many = sh.count > 2 * K;
+        __syncthreads();  // all have read it before anyone pushes again
+        const uint32_t least = many ? reached_by_k(sh, K) : 0u;
         if (least) tau = value_of(least);
-        __syncthreads();
       }
       continue;
     }
@@ -612,9 +683,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
 
 template <typename T, int NT>
 cudaError_t launch_nt(const LpParams& p, int rows, int ctas, cudaStream_t stream) {
+  constexpr int kRingBytes = NT == 256 ? 2 * kLpUnroll * NT * 16 : 0;
+  auto kern = token_logprobs_kernel<T, NT>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  static std::atomic<unsigned long long> attr_set{0};  // one bit per device
+  if (dev >= 64 || !(attr_set.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set.fetch_or(1ull << dev);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * ctas);
   cfg.blockDim = NT;
+  cfg.dynamicSmemBytes = kRingBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -624,7 +707,7 @@ cudaError_t launch_nt(const LpParams& p, int rows, int ctas, cudaStream_t stream
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = tvk::pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, p);
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 // CTAs per row: as many as keep all rows resident at once, but none with less than a vector per
