@@ -61,6 +61,12 @@ __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
 }
 
+// Asynchronous 16-byte copy global -> shared, and the thread's wait for all of its copies.
+__device__ __forceinline__ void copy16_async(uint4* dst, const uint4* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Two halves -> two e4m3 codes, nearest, ties to even.
 __device__ __forceinline__ uint32_t encode2h(uint32_t h) {
   uint32_t r;

@@ -16,17 +16,26 @@
 // says whether it is and which rows the block gets, and if so does the whole block,
 // one warp per (K or V, head).  So no two CTAs write one block and nothing depends on
 // their order, whatever the slots are; with prompts' runs of slots there is one
-// such token per block.  Reading all slots per block costs T^2 / block_size reads from L2: at 8,192
-// tokens about a third of the call (33 us for 50 MB of rows and codes), and what bounds calls of
-// more than some 30,000 rows.  Few tokens are latency: slot, other slots, rows, store, one
-// behind the other (64 rows of 4 heads of 64: 4.7 us, 256 of 8 of 128: 6.5 us).
+// such token per block.  A warp copies a block's rows to shared memory, all at once in flight, and
+// takes the maximum and the codes from there (from registers, two loads at a time and again
+// for the codes, 8,192 rows of 8 x 128 took 33 us instead of 22).
+//
+// Reading all slots per block costs T^2 / block_size reads from L2: at 8,192 tokens 4 of the 22 us (50 MB of
+// rows and codes, 2.3 TB/s), and what bounds calls of more than some 30,000 rows.  The rest
+// is issue slots (0.6 of them taken) and the barriers between a block's steps.  A CTA per token
+// up to 1,024 tokens, where the chain of loads counts (slot, other slots, rows, store, one behind
+// the other: 64 rows of 4 heads of 64 4.2 us, 256 of 8 of 128 5.9 us); beyond, 8 tokens a CTA
+// and two (K or V, head) a warp, which halves the reads of slots: 22.3 us, 16 tokens and one 23.9.
+#include <type_traits>
+
 #include "kv_cache_q8.cuh"
 
 namespace {
 
-constexpr int kWriteThreads = 256;
+constexpr int kWriteThreads = 256, kWriteCtas = 4;
+constexpr int kStage = 256;  // 16-byte vectors of rows that a warp holds in shared memory
 constexpr int kMaxBlockSize = 1024;
-constexpr int kFewTokens = 1024, kChunk = 16;  // tokens per CTA: one up to kFewTokens, else kChunk
+constexpr int kFewTokens = 1024, kChunk = 8;  // tokens per CTA: one up to kFewTokens, else kChunk
 
 struct WriteParams {
   const void *k, *v;           // [n_tokens, n_kv_heads, head_dim]
@@ -38,23 +47,41 @@ struct WriteParams {
   long long n_slots;
 };
 
-// Eight elements as they lie in memory, and as floats.
+// Eight elements as floats.
 template <typename T>
-struct Raw8 {
-  uint4 u[sizeof(T) / 2];
-};
-template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p) {
-  Raw8<T> r;
+__device__ __forceinline__ void to_floats(const uint4* u, float* f) {
+  uint4 r[sizeof(T) / 2];
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void to_floats(const Raw8<T>& r, float* f) {
-  const T* h = reinterpret_cast<const T*>(&r);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = u[i];
+  const T* h = reinterpret_cast<const T*>(r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = DT<T>::to_f(h[i]);
+}
+
+// Largest magnitude of the finite ones of eight elements and m.  |x| + 0 |x| is NaN where x is not
+// finite, and the maximum passes over NaN.
+template <typename T>
+__device__ __forceinline__ float amax8(const uint4* u, float m) {
+  if constexpr (sizeof(T) == 4) {
+    float f[8];
+    to_floats<T>(u, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaf(fabsf(f[e]), 0.f, fabsf(f[e])));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const uint4 r = *u;
+    const T2* h = reinterpret_cast<const T2*>(&r);
+    T2 zero, best;
+    zero.x = zero.y = DT<T>::from_f(0.f);
+    best = zero;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T2 x = __habs2(h[i]);
+      best = __hmax2(best, __hfma2(x, zero, x));
+    }
+    return fmaxf(m, fmaxf(DT<T>::to_f(best.x), DT<T>::to_f(best.y)));
+  }
 }
 
 __device__ __forceinline__ uint2 encode8(const float* f) {
@@ -67,7 +94,7 @@ __device__ __forceinline__ uint2 encode8(const float* f) {
 // Rows of D8 groups of 8 elements, walked 32 groups at a time by a warp.
 struct Walk8 {
   int row, c, drow, dc, D8;
-  __device__ Walk8(int lane, int D8_) : row(lane / D8_), c(lane % D8_), drow(32 / D8_), dc(32 % D8_), D8(D8_) {}
+  __device__ Walk8(int at, int D8_) : row(at / D8_), c(at % D8_), drow(32 / D8_), dc(32 % D8_), D8(D8_) {}
   __device__ void next() {
     row += drow;
     c += dc;
@@ -79,11 +106,13 @@ struct Walk8 {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteCtas) write_kv_q8_kernel(const WriteParams p) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int row_of[kMaxBlockSize];   // last token of the call for each slot of the block, or -1
-  __shared__ int2 rows[kMaxBlockSize];    // (slot in the block, token) of those there are
-  __shared__ int first, n_rows, cands[kChunk], n_cands;
+  __shared__ uint16_t rows[kMaxBlockSize];  // the slots of the block that get a row
+  __shared__ uint4 stage_s[kWriteThreads / 32][kStage];
+  __shared__ int first, n_rows, n_cands;
+  __shared__ int2 cands[kChunk];  // (token, its block)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bs = p.block_size;
   const int D = p.head_dim, D8 = D / 8, H = p.n_kv_heads;
   const size_t row_elems = (size_t)H * D;
@@ -91,18 +120,20 @@ __global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const Wri
     // the chunk's tokens that the token before them does not share the block with
     const int t = blockIdx.x * p.chunk + lane;
     bool cand = false;
+    long long blk = 0;
     if (lane < p.chunk && t < p.n_tokens) {
       const long long slot = p.slots[t], before = t > 0 ? p.slots[t - 1] : -1;
-      cand = slot >= 0 && slot < p.n_slots && (before < 0 || before / bs != slot / bs);
+      blk = slot / bs;
+      cand = slot >= 0 && slot < p.n_slots && (before < 0 || before / bs != blk);
     }
     const unsigned m = __ballot_sync(0xffffffffu, cand);
-    if (cand) cands[__popc(m & ((1u << lane) - 1u))] = t;
+    if (cand) cands[__popc(m & ((1u << lane) - 1u))] = make_int2(t, (int)blk);
     if (lane == 0) n_cands = __popc(m);
   }
   __syncthreads();
   for (int ci = 0; ci < n_cands; ++ci) {
-    const int t = cands[ci];
-    const long long blk = p.slots[t] / bs, base = blk * bs;
+    const int t = cands[ci].x, blk = cands[ci].y;
+    const long long base = (long long)blk * bs;
     __syncthreads();  // the block before is done with
     for (int i = tid; i < bs; i += kWriteThreads) row_of[i] = -1;
     if (tid == 0) {
@@ -129,7 +160,7 @@ __global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const Wri
     __syncthreads();
     if (first != t) continue;  // the same for all threads
     for (int i = tid; i < bs; i += kWriteThreads)
-      if (row_of[i] >= 0) rows[atomicAdd(&n_rows, 1)] = make_int2(i, row_of[i]);
+      if (row_of[i] >= 0) rows[atomicAdd(&n_rows, 1)] = (uint16_t)i;
     __syncthreads();
 
     const int n = n_rows;
@@ -142,36 +173,27 @@ __global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const Wri
       float old = started ? 0.f : *sp;
       if (!(old > 0.f && old < INFINITY)) old = 0.f;
 
-      // Both passes read the rows; the second finds them in L1.
-      constexpr int kInFlight = 2;  // loads: more would cost the fourth CTA on an SM, which is worth more
-      auto for_rows = [&](auto&& use) {
-        Walk8 w(lane, D8);
-        while (w.row < n) {
-          Raw8<T> r[kInFlight];
-          int2 at[kInFlight];  // slot in the block (-1: none), group of 8
+      // The rows in groups of 8 elements, as many at a time as the stage holds: all copies are in flight
+      // at once, and each lane reads back its own.  Only rows beyond the stage are fetched again for the second pass.
+      constexpr int kVecs = sizeof(T) / 2, kItems = kStage / kVecs;
+      uint4* stage = stage_s[warp] + lane * kVecs;
+      const int items = n * D8;
+      auto fetch = [&](int from) {
+        Walk8 w(from + lane, D8);
+        for (int i = lane; i < kItems && from + i < items; i += 32, w.next()) {
+          const T* src = x + (size_t)row_of[rows[w.row]] * row_elems + w.c * 8;
+          uint4* dst = stage + (i - lane) * kVecs;
 #pragma unroll
-          for (int k = 0; k < kInFlight; ++k) {
-            at[k].x = -1;
-            if (w.row < n) {
-              const int2 row = rows[w.row];
-              at[k] = make_int2(row.x, w.c);
-              r[k] = load8<T>(x + (size_t)row.y * row_elems + w.c * 8);
-            }
-            w.next();
-          }
-#pragma unroll
-          for (int k = 0; k < kInFlight; ++k)
-            if (at[k].x >= 0) use(r[k], at[k].x, at[k].y);
+          for (int k = 0; k < kVecs; ++k) q8::copy16_async(dst + k, reinterpret_cast<const uint4*>(src) + k);
         }
+        q8::wait_copies();
       };
       float amax = 0.f;
-      for_rows([&](const Raw8<T>& r, int, int) {
-        float f[8];
-        to_floats<T>(r, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (isfinite(f[e])) amax = fmaxf(amax, fabsf(f[e]));
-      });
+      for (int from = 0; from < items; from += kItems) {
+        fetch(from);
+#pragma unroll 4
+        for (int i = lane; i < kItems && from + i < items; i += 32) amax = amax8<T>(stage + (i - lane) * kVecs, amax);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const float now = fmaxf(old, q8::scale_for(amax));
@@ -182,16 +204,24 @@ __global__ void __launch_bounds__(kWriteThreads, 4) write_kv_q8_kernel(const Wri
       __syncwarp();  // every lane has read the old scale
       if (lane == 0) *sp = now;
 
-      for_rows([&](const Raw8<T>& r, int slot_in, int c) {
-        float f[8];
-        to_floats<T>(r, f);
+      auto encode_rows = [&](auto scaled) {
+        for (int from = 0; from < items; from += kItems) {
+          if (items > kItems) fetch(from);
+          Walk8 w(from + lane, D8);
+#pragma unroll 2
+          for (int i = lane; i < kItems && from + i < items; i += 32, w.next()) {
+            float f[8];
+            to_floats<T>(stage + (i - lane) * kVecs, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = pow2 ? f[e] * inv : __fdiv_rn(f[e], now);
-          f[e] = isfinite(f[e]) ? y : __int_as_float(0x7fffffff);
+            for (int e = 0; e < 8; ++e) f[e] = fmaf(f[e], 0.f, scaled(f[e]));  // NaN where f is not finite
+            *reinterpret_cast<uint2*>(codes + (size_t)rows[w.row] * row_elems + w.c * 8) = encode8(f);
+          }
         }
-        *reinterpret_cast<uint2*>(codes + (size_t)slot_in * row_elems + c * 8) = encode8(f);
-      });
+      };
+      if (pow2)
+        encode_rows([inv](float f) { return f * inv; });
+      else
+        encode_rows([now](float f) { return __fdiv_rn(f, now); });
 
       if (n < bs && (started || now != old)) {  // the block's other rows
         const float ratio = __fdiv_rn(old, now);
@@ -244,8 +274,9 @@ extern "C" int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t
                 "k, v, k_cache and v_cache must be 16-byte aligned");
   const WriteParams p{k, v, (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, slots, n_tokens, n_kv_heads,
                       head_dim, block_size, n_tokens > kFewTokens ? kChunk : 1, (long long)num_blocks * block_size};
-  // a warp per (K or V, head)
-  const dim3 grid((n_tokens + p.chunk - 1) / p.chunk, (2 * n_kv_heads + kWriteThreads / 32 - 1) / (kWriteThreads / 32));
+  // a warp per (K or V, head), in long calls per two of them
+  const int per_cta = kWriteThreads / 32 * (n_tokens > kFewTokens ? 2 : 1);
+  const dim3 grid((n_tokens + p.chunk - 1) / p.chunk, (2 * n_kv_heads + per_cta - 1) / per_cta);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
     case TVK_DTYPE_F16: TVK_CHECK_CUDA(tvk::launch_pdl(write_kv_q8_kernel<__half>, grid, kWriteThreads, 0, s, p)); break;
