@@ -250,11 +250,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     if row_stride < vocab:
         raise ValueError("rows of logits must not overlap")
     code = _lib.dtype_code(logits)
-    top_tokens = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device)
-    # one allocation for the three fp32 results
-    lp, ent, top = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=logits.device).split_with_sizes(
-        (rows, rows, rows * top_k))
-    top = top.view(rows, top_k)
+    # one allocation for the four results, each contiguous
+    room = tokens.new_empty(2 * rows * (1 + top_k))
+    values, n = room.view(torch.float32), 2 * rows
+    lp, ent = values.as_strided((rows,), (1,), 0), values.as_strided((rows,), (1,), rows)
+    top = values.as_strided((rows, top_k), (top_k, 1), n)
+    top_tokens = room.as_strided((rows, top_k), (top_k, 1), n + rows * top_k)
     rc = _lib.call_on(dev, _lib.lib().tvk_token_logprobs, logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(),
                       ent.data_ptr(), top.data_ptr(), top_tokens.data_ptr(), rows, vocab, row_stride, top_k, code,
                       _lib.raw_stream(dev))
