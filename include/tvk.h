@@ -273,7 +273,14 @@ int tvk_argmax(const void* logits, int32_t* out, int rows, int vocab, long long 
  */
 int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t* slots, void* k_cache, void* v_cache,
                           float* k_scale, float* v_scale, int n_tokens, int n_kv_heads, int head_dim,
-                          int num_blocks, int block_size, int dtype, void* stream);
+                          int num_blocks, int block_size, int dtype, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
+ * Bytes of scratch that call needs: 0 up to 8,192 tokens, else 8 per 32 of them.  It need not
+ * be zeroed, is 8-byte aligned and serves one stream at a time.
+ */
+size_t tvk_write_kv_q8_workspace_size(int n_tokens);
 
 /*
  * Bytes of scratch tvk_paged_decode_attention_q8 needs: a 256-byte header (the

@@ -305,6 +305,58 @@ def test_write_twice_changes_nothing(cuda):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("T", [8192, 8193, 30011])
+@pytest.mark.parametrize("kind", ["run", "reversed", "any", "same", "nothing", "prompts"])
+def test_write_of_many_rows(cuda, T, kind):
+    """Calls that look for a block's rows by classes of blocks, and the last that does not."""
+    n, bs = T // 16 + 40, 16
+
+    def prompts(rng):                       # runs over blocks in any order, each from a block's start, with skipped rows
+        blocks, out = list(rng.permutation(n)), []
+        while len(out) < T:
+            m = int(rng.integers(1, 400))
+            own = [blocks.pop() for _ in range(-(-m // bs))] if len(blocks) * bs > 400 else []
+            out += [int(b) * bs + o for b in own for o in range(bs)][:m] if own else [-1] * m
+        return out[:T]
+
+    make = prompts if kind == "prompts" else SLOTS[kind](n, bs, T)
+    _check_write(*_write_case(cuda, T, 1, 32, bs, n, torch.bfloat16, T, make))
+
+
+def test_long_writes_at_once_and_recorded(cuda):
+    """Long calls on two streams and from two graphs at the same time, each with a workspace of its own."""
+    from tinyvllm_b200 import layers
+    T, n = 20000, 1300
+    cs = [_write_case(cuda, T, 2, 64, 16, n, torch.float16, s, lambda rng: (rng.permutation(n - 1)[:, None] * 16 + np.arange(16)).reshape(-1)[:T].tolist()) for s in (1, 2)]
+    want = []
+    for x, codes, scale, slots in cs:
+        c, s = [t.clone() for t in codes], [t.clone() for t in scale]
+        layers.write_kv_slots_q8(x[0], x[1], slots, *c, *s)
+        want.append([t.view(torch.uint8).clone() for t in c])
+    streams, graphs, rec = [torch.cuda.Stream(), torch.cuda.Stream()], [], torch.cuda.Stream()
+    call = lambda c: layers.write_kv_slots_q8(c[0][0], c[0][1], c[3], *c[1], *c[2])
+    torch.cuda.synchronize()
+    for c in cs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=rec):
+            call(c)
+        graphs.append(g)
+    for use in (lambda i: call(cs[i]), lambda i: graphs[i].replay()):
+        for c in cs:
+            for t in c[1]:
+                t.view(torch.uint8).zero_()
+        torch.cuda.synchronize()
+        for _ in range(8):
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    use(i)
+        torch.cuda.synchronize()
+        for c, w in zip(cs, want):
+            started = torch.zeros(n, dtype=torch.bool, device=cuda)
+            started[c[3][c[3] % 16 == 0] // 16] = True
+            assert all(torch.equal(t.view(torch.uint8)[started], v[started]) for t, v in zip(c[1], w))
+
+
 # ------------------------------------------------------------------ how they are called
 def test_python_refusals(cuda):
     from tinyvllm_b200 import layers

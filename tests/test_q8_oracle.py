@@ -60,7 +60,7 @@ P = 1 << 20      # an aligned address that nothing reads: every call below is re
 
 
 def _decode(lib, **kw):
-    a = dict(q=P, k=P, v=P, ks=P, vs=P, bt=P, ctx=P, out=P, batch=2, hq=8, hkv=2, d=64, bs=16, nb=8, mb=4, mcl=-1, dt=1, ws=P, n=1 << 30)
+    a = dict(q=P, k=P, v=P, ks=P, vs=P, bt=P, ctx=P, out=P << 1, batch=2, hq=8, hkv=2, d=64, bs=16, nb=8, mb=4, mcl=-1, dt=1, ws=P, n=1 << 30)
     a.update(kw)
     rc = lib.tvk_paged_decode_attention_q8(*[a[k] for k in ("q", "k", "v", "ks", "vs", "bt", "ctx", "out", "batch", "hq", "hkv", "d", "bs",
                                                             "nb", "mb", "mcl", "dt", "ws", "n")], None)
@@ -72,7 +72,7 @@ def _decode(lib, **kw):
     (dict(k=P + 8), -1, "aligned"), (dict(batch=-1), -1, "batch"), (dict(hq=7), -1, "multiple"), (dict(hq=64), -1, "exceeds"),
     (dict(d=96), -2, "head_dim"), (dict(d=256), -2, "head_dim"), (dict(bs=0), -1, "positive"), (dict(dt=3), -1, "dtype"),
     (dict(ws=None), -4, "workspace"), (dict(n=4096), -4, "workspace"), (dict(ws=P + 4), -1, "aligned"),
-    (dict(mb=1 << 28), -1, "2^31"), (dict(batch=1 << 20, mb=1 << 20), -1, "32-bit"),
+    (dict(out=P), -1, "overlap"), (dict(out=P + 2032), -1, "overlap"), (dict(out=P - 16), -1, "overlap"), (dict(mb=1 << 28), -1, "2^31"), (dict(batch=1 << 20, mb=1 << 20), -1, "32-bit"),
 ])
 def test_decode_refuses(lib, kw, rc, say):
     got, msg = _decode(lib, **kw)
@@ -81,7 +81,7 @@ def test_decode_refuses(lib, kw, rc, say):
 
 def test_empty_calls_are_fine(lib):
     assert _decode(lib, batch=0, q=None, ws=None)[0] == 0
-    assert lib.tvk_write_kv_slots_q8(None, None, None, None, None, None, None, 0, 2, 64, 8, 16, 1, None) == 0
+    assert lib.tvk_write_kv_slots_q8(None, None, None, None, None, None, None, 0, 2, 64, 8, 16, 1, None, 0, None) == 0
     assert lib.tvk_token_logprobs(None, None, None, None, None, None, 0, 10, 10, 0, 1, None) == 0
 
 
@@ -90,9 +90,10 @@ def test_empty_calls_are_fine(lib):
     ((P + 2, P, P, P, P, P, P, 4, 2, 64, 8, 16, 1), -1, "aligned"), ((P, P, P, P, P, P, P, -1, 2, 64, 8, 16, 1), -1, "n_tokens"),
     ((P, P, P, P, P, P, P, 4, 2, 24, 8, 16, 1), -1, "head_dim"), ((P, P, P, P, P, P, P, 4, 2, 64, 8, 2048, 1), -2, "block_size"),
     ((P, P, P, P, P, P, P, 4, 0, 64, 8, 16, 1), -1, "positive"), ((P, P, P, P, P, P, P, 4, 2, 64, 8, 16, 7), -1, "dtype"),
+    ((P, P, P, P, P, P, P, 8193, 2, 64, 8, 16, 1), -4, "workspace"),
 ])
 def test_write_refuses(lib, args, rc, say):
-    assert lib.tvk_write_kv_slots_q8(*args, None) == rc
+    assert lib.tvk_write_kv_slots_q8(*args, None, 0, None) == rc
     assert say in lib.tvk_last_error().decode()
 
 

@@ -53,7 +53,8 @@ SIGNATURES = {
     "tvk_probe_mma_issue": (_c_int, [_c_int, _c_int, _c_void, _c_int, _c_void]),
     "tvk_probe_exp_unit": (_c_int, [_c_int, _c_int, _c_void, _c_int, _c_void, _c_void]),
     "tvk_stream_capture_id": (_c_int, [_c_void, _c_void]),
-    "tvk_write_kv_slots_q8": (_c_int, [_c_void] * 7 + [_c_int] * 6 + [_c_void]),
+    "tvk_write_kv_q8_workspace_size": (_c_size, [_c_int]),
+    "tvk_write_kv_slots_q8": (_c_int, [_c_void] * 7 + [_c_int] * 6 + [_c_void, _c_size, _c_void]),
     "tvk_paged_decode_q8_workspace_size": (_c_size, [_c_int] * 2),
     "tvk_paged_decode_attention_q8": (_c_int, [_c_void] * 8 + [_c_int] * 9 + [_c_void, _c_size, _c_void]),
     "tvk_token_logprobs": (_c_int, [_c_void] * 6 + [_c_int, _c_int, _c_int64, _c_int, _c_int, _c_void]),

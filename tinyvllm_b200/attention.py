@@ -72,11 +72,17 @@ def _workspace_q8(index: int, batch: int, n_kv_heads: int) -> torch.Tensor:
     if not _q8_fixed_bytes:
         _q8_fixed_bytes = L.tvk_paged_decode_q8_workspace_size(0, 0)
     nbytes = L.tvk_paged_decode_q8_workspace_size(batch, n_kv_heads)
-    ws = _capture_workspace(index, nbytes, "decode_q8", nbytes - _q8_fixed_bytes)
+    return call_workspace(index, nbytes, "decode_q8", nbytes - _q8_fixed_bytes)
+
+
+def call_workspace(index: int, nbytes: int, kind: str, zero_tail: int = 0) -> torch.Tensor:
+    """A workspace of at least ``nbytes`` for a call on the current stream of device ``index``:
+    the recorded graph's own, or the stream's (zeroed once)."""
+    ws = _capture_workspace(index, nbytes, kind, zero_tail)
     if ws is None:
-        ws = _workspaces.get((index, _lib.raw_stream(index), "decode_q8"))
+        ws = _workspaces.get((index, _lib.raw_stream(index), kind))
         if ws is None or ws.numel() < nbytes:
-            ws = _workspace(torch.device("cuda", index), nbytes, "decode_q8")
+            ws = _workspace(torch.device("cuda", index), nbytes, kind)
     return ws
 
 

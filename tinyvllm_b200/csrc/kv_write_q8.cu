@@ -21,8 +21,11 @@
 // for the codes, 8,192 rows of 8 x 128 took 33 us instead of 22).
 //
 // Reading all slots per block costs T^2 / block_size reads from L2: at 8,192 tokens 4 of the 22 us (50 MB of
-// rows and codes, 2.3 TB/s), and what bounds calls of more than some 30,000 rows.  The rest
-// is issue slots (0.6 of them taken) and the barriers between a block's steps.  A CTA per token
+// rows and codes, 2.3 TB/s).  Longer calls make a pass over the slots first that notes, for every 32 tokens, which
+// of 64 classes of blocks they write, and read only the slots of groups that may hold a block's
+// (8 x 128 fp16: 8,192 rows take 18.8 us either way, 4,096 17.1 instead of 15.4, 16,384 33 instead of 35, 131,072 259
+// instead of 538; smallest and largest block per group instead of classes: 821, blocks being anywhere in a pool).
+// The rest is issue slots (0.6 of them taken) and the barriers between a block's steps.  A CTA per token
 // up to 1,024 tokens, where the chain of loads counts (slot, other slots, rows, store, one behind
 // the other: 64 rows of 4 heads of 64 4.2 us, 256 of 8 of 128 5.9 us); beyond, 8 tokens a CTA
 // and two (K or V, head) a warp, which halves the reads of slots: 22.3 us, 16 tokens and one 23.9.
@@ -33,6 +36,7 @@
 namespace {
 
 constexpr int kWriteThreads = 256, kWriteCtas = 4;
+constexpr int kReadAll = 8192;  // beyond so many tokens a block's rows are looked for by classes of blocks
 constexpr int kStage = 256;  // 16-byte vectors of rows that a warp holds in shared memory
 constexpr int kMaxBlockSize = 1024;
 constexpr int kFewTokens = 1024, kChunk = 8;  // tokens per CTA: one up to kFewTokens, else kChunk
@@ -44,6 +48,7 @@ struct WriteParams {
   const int64_t* slots;  // [n_tokens]
   int n_tokens, n_kv_heads, head_dim, block_size;
   int chunk;  // tokens a CTA looks after
+  const uint2* classes;  // classes of the blocks of every 32 tokens, or null
   long long n_slots;
 };
 
@@ -105,6 +110,22 @@ struct Walk8 {
   }
 };
 
+// One of 64 classes of blocks.
+__device__ __forceinline__ int class_of(int blk) { return (int)(((uint32_t)blk * 0x9e3779b1u) >> 26); }
+
+// Which classes of blocks every 32 tokens write, a warp each.
+__global__ void __launch_bounds__(kWriteThreads) slot_classes_kernel(const int64_t* slots, int n_tokens, int block_size,
+                                                                     long long n_slots, uint2* classes) {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+  const int t = blockIdx.x * kWriteThreads + threadIdx.x;
+  const long long slot = t < n_tokens ? slots[t] : -1;
+  const bool in = slot >= 0 && slot < n_slots;
+  const int c = in ? class_of((int)(slot / block_size)) : 0;
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, in && c < 32 ? 1u << c : 0u);
+  const uint32_t hi = __reduce_or_sync(0xffffffffu, in && c >= 32 ? 1u << (c - 32) : 0u);
+  if ((threadIdx.x & 31) == 0 && t < n_tokens) classes[t / 32] = make_uint2(lo, hi);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) write_kv_q8_kernel(const WriteParams p) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
@@ -148,15 +169,35 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) write_kv_q8_kernel(
         if (i < t) atomicMin(&first, i);
       }
     };
+    if (p.classes) {
+      // only the groups of 32 tokens that write a block of this one's class
+      const int groups = (p.n_tokens + 31) / 32, c = class_of(blk);
+      constexpr int kAtOnce = 4;
+      for (int g0 = warp * 32; g0 < groups; g0 += kAtOnce * kWriteThreads) {
+        uint2 r[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int g = g0 + k * kWriteThreads + lane;
+          r[k] = g < groups ? p.classes[g] : make_uint2(0u, 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          for (unsigned m = __ballot_sync(0xffffffffu, ((c < 32 ? r[k].x : r[k].y) >> (c & 31)) & 1u); m; m &= m - 1) {
+            const int i = (g0 + k * kWriteThreads + __ffs(m) - 1) * 32 + lane;
+            if (i < p.n_tokens) look(p.slots[i], i);
+          }
+      }
+    }
     // two slots a load where they are aligned (an odd last one apart)
-    const int pairs = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0 ? p.n_tokens / 2 : 0;
+    const int to_read = p.classes ? 0 : p.n_tokens;
+    const int pairs = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0 ? to_read / 2 : 0;
 #pragma unroll 8
     for (int i = tid; i < pairs; i += kWriteThreads) {
       const longlong2 two = reinterpret_cast<const longlong2*>(p.slots)[i];
       look(two.x, 2 * i);
       look(two.y, 2 * i + 1);
     }
-    for (int i = 2 * pairs + tid; i < p.n_tokens; i += kWriteThreads) look(p.slots[i], i);
+    for (int i = 2 * pairs + tid; i < to_read; i += kWriteThreads) look(p.slots[i], i);
     __syncthreads();
     if (first != t) continue;  // the same for all threads
     for (int i = tid; i < bs; i += kWriteThreads)
@@ -256,9 +297,14 @@ bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
 }  // namespace
 
+extern "C" size_t tvk_write_kv_q8_workspace_size(int n_tokens) {
+  return n_tokens > kReadAll ? ((size_t)n_tokens + 31) / 32 * sizeof(uint2) : 0;
+}
+
 extern "C" int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t* slots, void* k_cache, void* v_cache,
                                      float* k_scale, float* v_scale, int n_tokens, int n_kv_heads, int head_dim,
-                                     int num_blocks, int block_size, int dtype, void* stream) {
+                                     int num_blocks, int block_size, int dtype, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
   TVK_CHECK_ARG(n_tokens >= 0, "negative n_tokens");
   TVK_CHECK_ARG(n_kv_heads > 0 && num_blocks > 0 && block_size > 0, "sizes must be positive");
   TVK_CHECK_ARG(head_dim > 0 && head_dim % 16 == 0, "head_dim must be a multiple of 16 (got %d)", head_dim);
@@ -272,12 +318,23 @@ extern "C" int tvk_write_kv_slots_q8(const void* k, const void* v, const int64_t
   TVK_CHECK_ARG(k && v && slots && k_cache && v_cache && k_scale && v_scale, "null pointer argument");
   TVK_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_cache) && aligned16(v_cache),
                 "k, v, k_cache and v_cache must be 16-byte aligned");
+  const size_t need = tvk_write_kv_q8_workspace_size(n_tokens);
+  if (need > 0 && (!workspace || workspace_bytes < need)) {
+    tvk::set_error("workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return TVK_ERR_WORKSPACE;
+  }
+  TVK_CHECK_ARG(need == 0 || (uintptr_t)workspace % 8 == 0, "workspace must be 8-byte aligned");
+  uint2* classes = need > 0 ? (uint2*)workspace : nullptr;
+  const long long n_slots = (long long)num_blocks * block_size;
   const WriteParams p{k, v, (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, slots, n_tokens, n_kv_heads,
-                      head_dim, block_size, n_tokens > kFewTokens ? kChunk : 1, (long long)num_blocks * block_size};
+                      head_dim, block_size, n_tokens > kFewTokens ? kChunk : 1, classes, n_slots};
   // a warp per (K or V, head), in long calls per two of them
   const int per_cta = kWriteThreads / 32 * (n_tokens > kFewTokens ? 2 : 1);
   const dim3 grid((n_tokens + p.chunk - 1) / p.chunk, (2 * n_kv_heads + per_cta - 1) / per_cta);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (classes)
+    TVK_CHECK_CUDA(tvk::launch_pdl(slot_classes_kernel, dim3((n_tokens + kWriteThreads - 1) / kWriteThreads), kWriteThreads, 0, s,
+                                   slots, n_tokens, block_size, n_slots, classes));
   switch (dtype) {
     case TVK_DTYPE_F16: TVK_CHECK_CUDA(tvk::launch_pdl(write_kv_q8_kernel<__half>, grid, kWriteThreads, 0, s, p)); break;
     case TVK_DTYPE_BF16:

@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .attention import call_workspace
 
 
 def _stream(dev):
@@ -165,9 +166,12 @@ def write_kv_slots_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     if not (k.is_contiguous() and v.is_contiguous() and slots.is_contiguous() and k_cache.is_contiguous()
             and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError("tensors must be contiguous")
-    rc = _lib.call_on(dev, _lib.lib().tvk_write_kv_slots_q8, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
+    L = _lib.lib()
+    need = L.tvk_write_kv_q8_workspace_size(T) if T > 1024 else 0     # a step's rows never need one
+    ws = call_workspace(dev, need, "write_q8").data_ptr() if need else 0
+    rc = _lib.call_on(dev, L.tvk_write_kv_slots_q8, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
                       k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, hkv, d, nb, bs,
-                      _lib.dtype_code(k), _lib.raw_stream(dev))
+                      _lib.dtype_code(k), ws, need, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "tvk_write_kv_slots_q8")
 
