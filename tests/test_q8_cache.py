@@ -128,6 +128,14 @@ def test_long_contexts_shared_by_ctas(cuda, dtype, B, ctx):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,d", [(1, 128), (4, 64), (7, 32), (16, 128)])
+def test_one_head_shared_by_all_ctas(cuda, dtype, hq, d):
+    """One KV head: every CTA has a part of its one unit (or of each few query heads), more parts than are joined at a time."""
+    c = _case(cuda, 1, hq, 1, d, 16, [70001], dtype, hq)
+    _check(c, _run(c, check=True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_many_sequences(cuda, dtype):
     rng = np.random.default_rng(4)
     ctx = [int(x) for x in rng.integers(0, 90, 700)]
