@@ -28,7 +28,7 @@
 
 namespace {
 
-constexpr int kSimtTile = 32;        // tokens the simt kernel stages at a time, and its tile of the work line
+constexpr int kSimtTile = 128;       // tokens the simt kernel's four warps go through at a time, and its tile of the work line
 constexpr int kSimtWhole = 2;        // its units of up to so many tiles are not cut
 constexpr int kTcTile = 128;         // the same for the tensor-core kernel: the rows of a matrix instruction
 constexpr int kTcWhole = 6;          // joining parts costs as much as 4 to 5 tiles in a row
@@ -56,6 +56,7 @@ struct Q8Params {
   float scale_log2;            // log2(e) / sqrt(head_dim)
   int n_stages;                // ring depth of the tensor-core kernel
   unsigned long long wait_ns;  // wall-time limit of every mbarrier wait
+  int dtype;                   // of q and out
   int drop_loads;              // wait-limit test: the producer issues nothing, so waits run out
 };
 
@@ -213,22 +214,65 @@ __device__ __forceinline__ float joined(const Q8Params& p, const Share& s, int n
   return A / L;
 }
 
+// Largest value of a warp (NaN only where all are).
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // -----------------------------------------------------------------------------
-// SIMT kernel: any query type, any block size; fp32 CUDA-core arithmetic on
-// 32-token tiles staged in shared memory.
+// SIMT kernel: any query type, any block size; fp32 CUDA-core arithmetic.
+//
+// Each of four warps goes through 32-token tiles of its own (every fourth of the share), whose
+// codes it copies to its part of shared memory: K of the next tile while it works on the weights,
+// V of the next while on the scores.  Scores: a lane per token, 16 codes at a time decoded to
+// registers and used for all GM query heads, whose elements are broadcast from shared memory (one
+// such read per four products).  Output: a lane per D / 32 dims, the weights (v_scale in them) broadcast
+// likewise.  Running maxima and sums are the warp's own; the four are put together at the end.
+//
+// Broadcast reads and products bound it: fp32, 16 sequences of 128-4096 tokens, 32/4 heads of 64 33 us, 8 with
+// 32/8 of 128 35 us (1.1 TB/s), 64 with 16/1 of 128 111 us, 4 sequences of 17-255 with 32/4 of 64 10.5 us.  (Codes decoded
+// to floats in shared memory by the whole CTA, a head per warp, took 60, 79, 174 and 14.5 us.)
 // -----------------------------------------------------------------------------
-template <typename T, int D>
+constexpr int kSimtWarpTile = 32;
+
+template <int D, int GM>
+struct SimtLayout {
+  static constexpr int kPitch = D + 16;  // bytes of a row of codes: rows of 8 lanes in different banks
+  static constexpr int kCodes = kSimtWarpTile * kPitch;
+  static constexpr int kWarp = 2 * kCodes + 2 * kSimtWarpTile * 4 + kSimtWarpTile * GM * 4;  // K, V, scales, weights
+  static constexpr int kBytes = GM * D * 4 + 4 * kWarp;
+  static_assert(GM * D * 4 + GM * 8 <= kWarp, "a warp's sums take the place of its tiles");
+};
+
+__device__ __forceinline__ float load_as_float(const void* x, size_t i, int dtype) {
+  if (dtype == TVK_DTYPE_F32) return static_cast<const float*>(x)[i];
+  if (dtype == TVK_DTYPE_F16) return DT<__half>::to_f(static_cast<const __half*>(x)[i]);
+  return DT<__nv_bfloat16>::to_f(static_cast<const __nv_bfloat16*>(x)[i]);
+}
+__device__ __forceinline__ void store_from_float(void* x, size_t i, float v, int dtype) {
+  if (dtype == TVK_DTYPE_F32)
+    static_cast<float*>(x)[i] = v;
+  else if (dtype == TVK_DTYPE_F16)
+    static_cast<__half*>(x)[i] = DT<__half>::from_f(v);
+  else
+    static_cast<__nv_bfloat16*>(x)[i] = DT<__nv_bfloat16>::from_f(v);
+}
+
+template <int D, int GM>
 __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int DP = D + 4;
-  constexpr int MAXK = kMaxGroup * D / 128;
-  __shared__ __align__(16) float qs[kMaxGroup * D];
-  __shared__ __align__(16) float ks[kSimtTile][DP];
-  __shared__ __align__(16) float vs[kSimtTile][DP];
-  __shared__ float ps[kMaxGroup][kSimtTile];
-  __shared__ float corr_s[kMaxGroup], mfin[kMaxGroup], lfin[kMaxGroup];
+  using L = SimtLayout<D, GM>;
+  constexpr int DV = D / 32;
+  extern __shared__ __align__(16) uint8_t simt_smem[];
   __shared__ int flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* qs = reinterpret_cast<float*>(simt_smem);  // [GM][D]
+  uint8_t* mine = simt_smem + GM * D * 4 + warp * L::kWarp;
+  uint8_t* codes[2] = {mine, mine + L::kCodes};
+  float* scales = reinterpret_cast<float*>(mine + 2 * L::kCodes);  // [K, V][token]
+  float* ps = scales + 2 * kSimtWarpTile;                          // [token][GM]
   const int G = p.group, bs = p.block_size, Hkv = p.n_kv_heads;
   using Walk = Walker<kSimtTile, kSimtWhole>;
   Cut cut;
@@ -238,118 +282,166 @@ __global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Param
   w.seek(p, cut, Hkv, blockIdx.x, lane);
   Share s;
   while (w.next(p, cut, Hkv, s)) {
-    T* out = reinterpret_cast<T*>(p.out) + ((size_t)s.b * p.n_heads + s.h * G) * D;
+    const size_t out0 = ((size_t)s.b * p.n_heads + s.h * G) * D;
     if (s.ctx == 0) {
-      for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(0.f);
+      for (int i = tid; i < G * D; i += 128) store_from_float(p.out, out0 + i, 0.f, p.dtype);
       continue;
     }
     __syncthreads();
-    const T* q = reinterpret_cast<const T*>(p.q) + ((size_t)s.b * p.n_heads + s.h * G) * D;
-    for (int i = tid; i < G * D; i += 128) qs[i] = DT<T>::to_f(q[i]);
+    for (int i = tid; i < GM * D; i += 128) qs[i] = i < G * D ? load_as_float(p.q, out0 + i, p.dtype) : 0.f;
+    __syncthreads();
     const int32_t* bt = p.block_tables + (size_t)s.b * p.max_blocks;
-    float acc[MAXK];
+    const int step = 4 * kSimtWarpTile;
+    // this lane's block of the tile at t0, -1 where there is none
+    auto block_of = [&](int t0) -> int {
+      const int blk = t0 + lane < s.tok1 ? __ldg(bt + (t0 + lane) / bs) : -1;
+      return blk < p.num_blocks ? blk : -1;
+    };
+    // K (kv 0) or V codes and scales of the tile at t0, one group of copies; zeros where there are none
+    auto issue = [&](int kv, int t0, int blk) {
+      const uint8_t* pool = kv ? p.v_cache : p.k_cache;
+      constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // 16-byte chunks of a row, rows at a time
+      const size_t row = ((size_t)(blk < 0 ? 0 : blk) * bs + (t0 + lane) % bs) * Hkv + s.h;
 #pragma unroll
-    for (int k = 0; k < MAXK; ++k) acc[k] = 0.f;
-    float m_own[kMaxGroup / 4], l_own[kMaxGroup / 4];  // heads warp, warp + 4, ...
+      for (int r = 0; r < kSimtWarpTile; r += kRows) {
+        const int t = r + lane / kChunks;
+        const size_t at = __shfl_sync(0xffffffffu, (unsigned long long)row, t);
+        const bool live = __shfl_sync(0xffffffffu, blk, t) >= 0;
+        q8::copy16_async_or_zeros(ptx::smem_u32(codes[kv] + t * L::kPitch + lane % kChunks * 16), pool + at * D + lane % kChunks * 16, live);
+      }
+      const float* src = kv ? p.v_scale : p.k_scale;
+      q8::copy4_async(ptx::smem_u32(scales + kv * kSimtWarpTile + lane), blk >= 0 ? src + (size_t)blk * Hkv + s.h : src, blk >= 0);
+      q8::commit_copies();
+    };
+    float acc[GM][DV], m[GM], l[GM];
 #pragma unroll
-    for (int i = 0; i < kMaxGroup / 4; ++i) {
-      m_own[i] = -INFINITY;
-      l_own[i] = 0.f;
+    for (int h = 0; h < GM; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int k = 0; k < DV; ++k) acc[h][k] = 0.f;
     }
-    for (int t0 = s.tok0; t0 < s.tok1; t0 += kSimtTile) {
-      __syncthreads();
-      for (int i = tid; i < kSimtTile * (D / 4); i += 128) {
-        const int t = i / (D / 4), d4 = (i % (D / 4)) * 4;
-        float kf[4] = {0.f, 0.f, 0.f, 0.f}, vf[4] = {0.f, 0.f, 0.f, 0.f};
-        const int tok = t0 + t;
-        if (tok < s.tok1) {
-          const int blk = __ldg(bt + tok / bs);
-          if (blk >= 0 && blk < p.num_blocks) {
-            const size_t off = (((size_t)blk * bs + tok % bs) * Hkv + s.h) * D + d4;
-            q8::decode4(*reinterpret_cast<const uint32_t*>(p.k_cache + off), kf);
-            q8::decode4(*reinterpret_cast<const uint32_t*>(p.v_cache + off), vf);
-            const float sk = p.k_scale[(size_t)blk * Hkv + s.h], sv = p.v_scale[(size_t)blk * Hkv + s.h];
+    const int first = s.tok0 + warp * kSimtWarpTile;
+    int blk = first < s.tok1 ? block_of(first) : -1;
+    if (first < s.tok1) {
+      issue(0, first, blk);
+      issue(1, first, blk);
+    }
+    for (int t0 = first; t0 < s.tok1; t0 += step) {
+      const int next = block_of(t0 + step);  // all -1 behind the end: the copies are zeros that nobody reads
+      q8::wait_copies_but<1>();
+      __syncwarp();
+      float x[GM];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              kf[e] *= sk;
-              vf[e] *= sv;
-            }
+      for (int h = 0; h < GM; ++h) x[h] = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < D; d += 16) {
+        const uint4 c = *reinterpret_cast<const uint4*>(codes[0] + lane * L::kPitch + d);
+        float f[16];
+        q8::decode4(c.x, f);
+        q8::decode4(c.y, f + 4);
+        q8::decode4(c.z, f + 8);
+        q8::decode4(c.w, f + 12);
+#pragma unroll
+        for (int h = 0; h < GM; ++h)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 q4 = *reinterpret_cast<const float4*>(qs + h * D + d + e);
+            x[h] = fmaf(q4.x, f[e], x[h]);
+            x[h] = fmaf(q4.y, f[e + 1], x[h]);
+            x[h] = fmaf(q4.z, f[e + 2], x[h]);
+            x[h] = fmaf(q4.w, f[e + 3], x[h]);
+          }
+      }
+      const float sk = scales[lane] * p.scale_log2;
+      const bool live = t0 + lane < s.tok1;
+      __syncwarp();  // every lane has read K and its scale
+      issue(0, t0 + step, next);
+      float corr[GM];
+      q8::wait_copies_but<1>();
+      const float sv = scales[kSimtWarpTile + lane];
+#pragma unroll
+      for (int h = 0; h < GM; ++h) {
+        x[h] = live ? x[h] * sk : -INFINITY;
+        const float mn = fmaxf(m[h], warp_max(x[h]));
+        corr[h] = exp2f(m[h] - mn);
+        m[h] = mn;
+        const float pv = exp2f(x[h] - mn);
+        l[h] = fmaf(l[h], corr[h], pv);
+        x[h] = live ? pv * sv : 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < GM; h += 4)
+        *reinterpret_cast<float4*>(ps + lane * GM + h) = make_float4(x[h], x[h + 1], x[h + 2], x[h + 3]);
+      __syncwarp();  // weights and V are there
+#pragma unroll
+      for (int h = 0; h < GM; ++h)
+#pragma unroll
+        for (int k = 0; k < DV; ++k) acc[h][k] *= corr[h];
+#pragma unroll 2
+      for (int t = 0; t < kSimtWarpTile; ++t) {
+        const uint8_t* at = codes[1] + t * L::kPitch + lane * DV;
+        const uint32_t c = DV == 4 ? *reinterpret_cast<const uint32_t*>(at) : DV == 2 ? *reinterpret_cast<const uint16_t*>(at) : *at;
+        float f[4];
+        q8::decode4(c, f);
+#pragma unroll
+        for (int h = 0; h < GM; h += 4) {
+          const float4 w4 = *reinterpret_cast<const float4*>(ps + t * GM + h);
+#pragma unroll
+          for (int k = 0; k < DV; ++k) {
+            acc[h][k] = fmaf(w4.x, f[k], acc[h][k]);
+            acc[h + 1][k] = fmaf(w4.y, f[k], acc[h + 1][k]);
+            acc[h + 2][k] = fmaf(w4.z, f[k], acc[h + 2][k]);
+            acc[h + 3][k] = fmaf(w4.w, f[k], acc[h + 3][k]);
           }
         }
-        *reinterpret_cast<float4*>(&ks[t][d4]) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-        *reinterpret_cast<float4*>(&vs[t][d4]) = make_float4(vf[0], vf[1], vf[2], vf[3]);
       }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kMaxGroup / 4; ++i) {
-        const int gh = warp + 4 * i;
-        if (gh < G) {
-          float x = 0.f;
-#pragma unroll 8
-          for (int d = 0; d < D; d += 4) {
-            const float4 kk = *reinterpret_cast<const float4*>(&ks[lane][d]);
-            const float4 qq = *reinterpret_cast<const float4*>(&qs[gh * D + d]);
-            x = fmaf(qq.x, kk.x, x);
-            x = fmaf(qq.y, kk.y, x);
-            x = fmaf(qq.z, kk.z, x);
-            x = fmaf(qq.w, kk.w, x);
-          }
-          x = (t0 + lane < s.tok1) ? x * p.scale_log2 : -INFINITY;
-          float mx = x;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float mn = fmaxf(m_own[i], mx);
-          const float corr = exp2f(m_own[i] - mn);
-          const float pv = exp2f(x - mn);
-          float sum = pv;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          l_own[i] = l_own[i] * corr + sum;
-          m_own[i] = mn;
-          ps[gh][lane] = pv;
-          if (lane == 0) corr_s[gh] = corr;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < MAXK; ++k) {
-        const int idx = tid + 128 * k;
-        if (idx < G * D) {
-          const int gh = idx / D, d = idx % D;
-          float a = acc[k] * corr_s[gh];
-#pragma unroll 8
-          for (int t = 0; t < kSimtTile; ++t) a = fmaf(ps[gh][t], vs[t][d], a);
-          acc[k] = a;
-        }
-      }
+      __syncwarp();  // every lane has read V and the weights
+      issue(1, t0 + step, next);
     }
+    // The warps' sums, relative to each warp's maxima, in place of its tiles.
+    q8::wait_copies();
+    __syncwarp();
+    float* sums = reinterpret_cast<float*>(mine);  // [GM][D], then (maximum, sum) of every head
 #pragma unroll
-    for (int i = 0; i < kMaxGroup / 4; ++i) {
-      const int gh = warp + 4 * i;
-      if (gh < G && lane == 0) {
-        mfin[gh] = m_own[i];
-        lfin[gh] = l_own[i];
+    for (int h = 0; h < GM; ++h) {
+      float sum = l[h];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+      for (int k = 0; k < DV; ++k) sums[h * D + lane * DV + k] = acc[h][k];
+      if (lane == 0) {
+        sums[GM * D + h * 2] = m[h];
+        sums[GM * D + h * 2 + 1] = sum;
       }
-    }
-    // the query rows are done with: their place takes the output sums
-#pragma unroll
-    for (int k = 0; k < MAXK; ++k) {
-      const int idx = tid + 128 * k;
-      if (idx < G * D) qs[idx] = acc[k];
     }
     __syncthreads();
-    if (s.n_parts == 1) {
-      for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(qs[i] / lfin[i / D]);
-      continue;
+    float* part = s.n_parts == 1 ? nullptr : part_slot(p, s.piece, s.piece == s.first_piece);
+    const float* all = reinterpret_cast<const float*>(simt_smem + GM * D * 4);
+    constexpr int kStride = L::kWarp / 4;
+    for (int i = tid; i < G * D; i += 128) {
+      const int h = i / D;
+      float M = -INFINITY, A = 0.f, Ls = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, all[k * kStride + GM * D + h * 2]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = exp2f(all[k * kStride + GM * D + h * 2] - M);
+        A = fmaf(all[k * kStride + i], f, A);
+        Ls = fmaf(all[k * kStride + GM * D + h * 2 + 1], f, Ls);
+      }
+      if (part) {
+        __stcg(part + i, A);
+        if (i % D == 0) {
+          __stcg(part + G * D + h * 2, M);
+          __stcg(part + G * D + h * 2 + 1, Ls);
+        }
+      } else {
+        store_from_float(p.out, out0 + i, A / Ls, p.dtype);
+      }
     }
-    float* mine = part_slot(p, s.piece, s.piece == s.first_piece);
-    for (int i = tid; i < G * D; i += 128) __stcg(mine + i, qs[i]);
-    for (int i = tid; i < G; i += 128) {
-      __stcg(mine + G * D + i * 2, mfin[i]);
-      __stcg(mine + G * D + i * 2 + 1, lfin[i]);
-    }
-    if (last_to_arrive(p, s, s.b * Hkv + s.h, &flag, tid, [] { __syncthreads(); }))
-      for (int i = tid; i < G * D; i += 128) out[i] = DT<T>::from_f(joined(p, s, G * D, i, i / D));
+    if (part && last_to_arrive(p, s, s.b * Hkv + s.h, &flag, tid, [] { __syncthreads(); }))
+      for (int i = tid; i < G * D; i += 128) store_from_float(p.out, out0 + i, joined(p, s, G * D, i, i / D), p.dtype);
   }
 }
 
@@ -468,13 +560,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsign
 // bytes that only the matrix unit reads, after a proxy fence (which is ordered behind it).
 __device__ __forceinline__ void store_byte(uint32_t addr, uint32_t x) {
   asm volatile("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tst.shared.u8 [%0], h;\n\t}" ::"r"(addr), "r"(x));
-}
-
-// Largest value of a warp (NaN only where all are).
-__device__ __forceinline__ float warp_max(float x) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 template <typename T, int D, int GP>
@@ -1083,19 +1168,45 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   }
 }
 
-template <typename T>
-int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
+// Lets a kernel have its dynamic shared memory, once per device.  A, B: so that each kernel has its own record.
+template <int A, int B, typename K>
+int allow_smem(K kern, int bytes) {
+  int dev = 0;
+  TVK_CHECK_CUDA(cudaGetDevice(&dev));
+  static std::atomic<unsigned long long> set{0};  // one bit per device
+  if (dev >= 64 || !(set.load() >> dev & 1)) {
+    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) set.fetch_or(1ull << dev);
+  }
+  return TVK_OK;
+}
+
+template <int D, int GM>
+int launch_simt_gm(const Q8Params& p, cudaStream_t stream) {
+  using L = SimtLayout<D, GM>;
+  auto kern = paged_decode_q8_simt_kernel<D, GM>;
+  const int rc = allow_smem<D, GM>(kern, L::kBytes);
+  if (rc != TVK_OK) return rc;
   const long long most = (long long)p.batch * p.n_kv_heads * (tiles_of(p.max_ctx_tokens, kSimtTile) + kUnitTiles);
   const int grid = (int)(most < kSimtCtas ? most : kSimtCtas);
-  switch (head_dim) {
-    case 32: TVK_CHECK_CUDA(tvk::launch_pdl(paged_decode_q8_simt_kernel<T, 32>, grid, 128, 0, stream, p)); break;
-    case 64: TVK_CHECK_CUDA(tvk::launch_pdl(paged_decode_q8_simt_kernel<T, 64>, grid, 128, 0, stream, p)); break;
-    default: TVK_CHECK_CUDA(tvk::launch_pdl(paged_decode_q8_simt_kernel<T, 128>, grid, 128, 0, stream, p)); break;
-  }
+  TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, 128, L::kBytes, stream, p));
   TVK_CHECK_LAUNCH("paged_decode_q8_simt");
   return TVK_OK;
 }
 
+template <int D>
+int launch_simt_d(const Q8Params& p, cudaStream_t stream) {
+  if (p.group <= 4) return launch_simt_gm<D, 4>(p, stream);
+  return p.group <= 8 ? launch_simt_gm<D, 8>(p, stream) : launch_simt_gm<D, 16>(p, stream);
+}
+
+int launch_simt(const Q8Params& p, int head_dim, cudaStream_t stream) {
+  switch (head_dim) {
+    case 32: return launch_simt_d<32>(p, stream);
+    case 64: return launch_simt_d<64>(p, stream);
+    default: return launch_simt_d<128>(p, stream);
+  }
+}
 
 template <typename T, int D, int GP>
 int launch_tc(const Q8Params& p, cudaStream_t stream) {
@@ -1153,7 +1264,7 @@ int launch_tc(const Q8Params& p, cudaStream_t stream) {
 template <typename T>
 int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
   const int bs = p.block_size;
-  if (!(bs == 8 || bs == 16 || bs == 32 || bs == 64 || bs % kTcTile == 0)) return launch_simt<T>(p, head_dim, stream);
+  if (!(bs == 8 || bs == 16 || bs == 32 || bs == 64 || bs % kTcTile == 0)) return launch_simt(p, head_dim, stream);
   if (head_dim == 32) return launch_tc<T, 32, 4>(p, stream);
   const int pairs = head_dim == 64 ? (p.n_kv_heads + 1) / 2 : p.n_kv_heads;
   const long long units = (long long)p.batch * pairs * ((p.group + 3) / 4);
@@ -1183,7 +1294,7 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
                 kMaxGroup);
   TVK_CHECK_ARG(block_size > 0 && num_blocks > 0 && max_blocks > 0,
                 "block_size, num_blocks and max_blocks must be positive");
-  TVK_CHECK_ARG((long long)max_blocks * block_size < 0x7fffffffLL, "a table spans more than 2^31 tokens");
+  TVK_CHECK_ARG((long long)max_blocks * block_size <= 0x7fffff00LL, "a table spans more than 2^31 - 256 tokens");
   TVK_CHECK_ARG((long long)batch * n_kv_heads * ((long long)max_blocks * block_size / kSimtTile + 1 + kUnitTiles) < 0x7fffffffLL,
                 "batch x KV heads x table tiles exceeds the 32-bit work index");
   TVK_CHECK_ARG(dtype == TVK_DTYPE_F32 || dtype == TVK_DTYPE_F16 || dtype == TVK_DTYPE_BF16, "unknown dtype %d", dtype);
@@ -1232,6 +1343,7 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
     blocks = cut < max_blocks ? cut : max_blocks;
   }
   p.max_ctx_tokens = blocks * block_size;
+  p.dtype = dtype;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)head_dim));
   const tvk::WaitTest wt = tvk::take_wait_test();
   p.wait_ns = wt.armed ? wt.limit_ns : tvk::kDefaultWaitNs;
@@ -1240,6 +1352,6 @@ extern "C" int tvk_paged_decode_attention_q8(const void* q, const void* k_cache,
   switch (dtype) {
     case TVK_DTYPE_F16: return launch_16bit<__half>(p, head_dim, s);
     case TVK_DTYPE_BF16: return launch_16bit<__nv_bfloat16>(p, head_dim, s);
-    default: return launch_simt<float>(p, head_dim, s);
+    default: return launch_simt(p, head_dim, s);
   }
 }
