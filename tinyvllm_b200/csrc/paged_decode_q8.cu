@@ -33,7 +33,7 @@ constexpr int kSimtWhole = 2;        // its units of up to so many tiles are not
 constexpr int kTcTile = 128;         // the same for the tensor-core kernel: the rows of a matrix instruction
 constexpr int kTcWhole = 6;          // joining parts costs as much as 4 to 5 tiles in a row
 constexpr int kMaxGroup = 16;        // query heads per KV head
-constexpr int kSimtCtas = 592;       // four CTAs on each of 148 SMs
+constexpr int kSimtCtas = 592;       // four CTAs on each of 148 SMs (two at 16 query heads: the second half follows)
 constexpr int kTcCtas = 296;         // two CTAs on each SM
 constexpr int kMaxPieces = kSimtCtas;
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
@@ -232,7 +232,7 @@ __device__ __forceinline__ float warp_max(float x) {
 // likewise.  Running maxima and sums are the warp's own; the four are put together at the end.
 //
 // Broadcast reads and products bound it: fp32, 16 sequences of 128-4096 tokens, 32/4 heads of 64 33 us, 8 with
-// 32/8 of 128 35 us (1.1 TB/s), 64 with 16/1 of 128 111 us, 4 sequences of 17-255 with 32/4 of 64 10.5 us.  (Codes decoded
+// 32/8 of 128 35 us (1.1 TB/s), 64 with 16/1 of 128 107 us, 4 sequences of 17-255 with 32/4 of 64 9.2 us.  (Codes decoded
 // to floats in shared memory by the whole CTA, a head per warp, took 60, 79, 174 and 14.5 us.)
 // -----------------------------------------------------------------------------
 constexpr int kSimtWarpTile = 32;
@@ -260,8 +260,9 @@ __device__ __forceinline__ void store_from_float(void* x, size_t i, float v, int
     static_cast<__nv_bfloat16*>(x)[i] = DT<__nv_bfloat16>::from_f(v);
 }
 
+// CTAs on an SM: four; two with the sums of 16 heads (64 sequences with 16/1 heads take 118 us with three and 107 with two).
 template <int D, int GM>
-__global__ void __launch_bounds__(128) paged_decode_q8_simt_kernel(const Q8Params p) {
+__global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_kernel(const Q8Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   using L = SimtLayout<D, GM>;
   constexpr int DV = D / 32;
