@@ -77,16 +77,10 @@ __device__ __forceinline__ void wait_copies_but() {
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Two halves -> two e4m3 codes, nearest, ties to even.
-__device__ __forceinline__ uint32_t encode2h(uint32_t h) {
+// Two halves -> two e5m2 codes, nearest, ties to even.
+__device__ __forceinline__ uint32_t encode2h_e5m2(uint32_t h) {
   uint32_t r;
-  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f16x2 c, %1;\n\tcvt.u32.u16 %0, c;\n\t}" : "=r"(r) : "r"(h));
-  return r;
-}
-// Two e4m3 codes (low 16 bits) -> two halves.
-__device__ __forceinline__ uint32_t decode2h(uint32_t codes) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(codes));
+  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e5m2x2.f16x2 c, %1;\n\tcvt.u32.u16 %0, c;\n\t}" : "=r"(r) : "r"(h));
   return r;
 }
 __device__ __forceinline__ uint32_t sub2h(uint32_t a, uint32_t b) {

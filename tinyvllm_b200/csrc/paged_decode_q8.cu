@@ -460,8 +460,13 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
 //  * a query row, scaled by a power of two to a maximum in [2^7, 2^8), is
 //    q1 + q2 + q3 + 2^-8 q4, each part the e4m3 of what is left: 4 significant bits
 //    a part, exact for fp16 and bf16 down to 2^-18 of 2^7, i.e. 2^-25 of the maximum;
-//  * a weight 2^(s + log2 v_scale - M), at most 2^8, is rounded to a half and is
-//    p1 + p2 + 2^-8 p3: exact down to 2^-18, where the largest counts as 2^4..2^8.
+//  * a weight 2^(s + log2 v_scale - M), at most 2^15, is p1 + p2 + 2^-8 (p3 + p4), each part the
+//    e5m2 of what is left: three significant bits and the sign of the rest make four bits a part, and
+//    e5m2's five exponent bits reach from 2^15 to 2^-16, so that a long tail behind one heavy
+//    token counts.  After p1 what is left is a half (2^-15 of the weight, 2^-25 at least), which the
+//    others hold exactly; the largest weight counts as 2^11..2^15.  (Three parts in e4m3, the first of a
+//    weight as a half, end at 2^-23 of the largest: weights below that, nearly all of a long tail, were
+//    lost, and the output was off by up to half of sum p|v|.)
 // The matrix unit sums in fp32.  So nothing is converted per K/V element: the work of
 // the CUDA cores is per (token, query head).  (Decoding the codes to halves for
 // mma.sync took 470 instructions per 16 tokens and 265 us where this took 218 us in
@@ -470,9 +475,10 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
 //
 // Now that call takes 184-198 us (from box to box), 5.7-6.1 TB/s of codes and scales, 0.87-0.92
 // of the measured copy rate: memory bounds units of 4 heads.  With 8 heads a unit
-// 5.5 TB/s, with 16 2.9 TB/s (32/4 and 32/2 heads of 128, the same sequences):
+// 5.3 TB/s, with 16 2.6 TB/s (32/4 and 32/2 heads of 128, the same sequences):
 // there the softmax warps' work per (token, query head) bounds it, about half of that
-// the three parts of a weight and their byte stores.
+// the parts of a weight and their byte stores.  (The fourth part costs nothing at 4 heads a unit, 3 % at
+// 8 and 10 % at 16: 102.9 -> 106.4 and 99.6 -> 110.2 us.)
 //
 // Roles: warp 0 streams K tiles (TMA) and their scales (4-byte asynchronous
 // copies), warp 3 V; warp 1 issues the products; warp 2 splits the query rows of the next share;
@@ -482,21 +488,22 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
 // them, K(0) K(1) V(0) K(2) V(1) ..., so that a K tile's slot is free again as soon as
 // its S^T is there and not only after the weights and P.V.
 // M and the reference R of the sums are per query head, the same in all threads.
-// They move only when a weight would pass 2^8 (or a sum's term 2^64); then O^T is rescaled.
+// They move only when a weight would pass 2^15 (or a sum's term 2^64); then O^T is rescaled.
 // -----------------------------------------------------------------------------
 constexpr int kTcThreads = 256;
 // Tiles whose scales are kept.  A producer writes a tile's scales once it has the tile's slot, which is free when
 // the product of the tile at least (kSlots - 1) / 2 before is done; S^T being double, the softmax is at most two
 // tiles behind that: 7 slots make 5 tiles in all.
 constexpr int kScaleRing = 8;
-constexpr float kLowPart = 0.00390625f;
+constexpr float kLowPart = 0.00390625f;  // 2^-8
+constexpr float kTopWeight = 11.f, kMostWeight = 15.f;  // log2 of what the largest weight counts as: when a reference is set, and at most
 
 template <int D, int GP>
 struct TcLayout {
   static constexpr int HP = 128 / D;
   static constexpr int HG = HP * GP;                    // query heads of a unit
   static constexpr int NS = 4 * GP;                     // columns of S^T of one KV head: (part, head)
-  static constexpr int NO = (3 * HG + 15) / 16 * 16;    // columns of O^T: (part, KV head, head)
+  static constexpr int NO = 4 * HG;                     // columns of O^T: (part, KV head, head)
   static constexpr int kOCol = 2 * HP * NS;             // after two buffers of S^T
   static constexpr int kTmemCols = kOCol + NO <= 64 ? 64 : kOCol + NO <= 128 ? 128 : 256;
   static constexpr int kSlot = kTcTile * 128;           // K or V codes of a tile
@@ -538,6 +545,22 @@ __device__ __forceinline__ void split_query(float (&x)[4], uint32_t (&w)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] -= f[i];
   }
+}
+
+// Two weights (neighbouring heads of a token) -> p1, p2, 2^8 p3 and 2^8 p4 of both, e5m2, two bytes each.  An e5m2 is the
+// upper byte of a half.  The first remainder is exact in fp32 and is rounded to a half; from there all is exact.
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t (&c)[4]) {
+  auto as_halves = [](uint32_t codes) { return __byte_perm(codes, 0u, 0x1404); };
+  c[0] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E5M2);
+  uint32_t h = as_halves(c[0]);
+  const float2 top = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  uint32_t r = DT<__half>::pack2(a - top.x, b - top.y);
+  c[1] = q8::encode2h_e5m2(r);
+  r = q8::sub2h(r, as_halves(c[1]));
+  const __half2 up = __hmul2(*reinterpret_cast<const __half2*>(&r), __float2half2_rn(256.f));
+  r = *reinterpret_cast<const uint32_t*>(&up);
+  c[2] = q8::encode2h_e5m2(r);
+  c[3] = q8::encode2h_e5m2(q8::sub2h(r, as_halves(c[2])));
 }
 
 // Or of a flag over the 128 threads of warps 4-7.
@@ -733,7 +756,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   } else if (warp == 1) {
     // ---------------- matrix issue: S^T of a tile, then P.V of the one before ----------------
     constexpr uint32_t idesc_s = umma::idesc_e4m3(128, L::NS, false);
-    constexpr uint32_t idesc_o = umma::idesc_e4m3(128, L::NO, true);
+    constexpr uint32_t idesc_o = umma::idesc_e4m3(128, L::NO, true, true);
     uint32_t it = 0, share = 0;
     bool ok = true;
     // The P.V that is due: tile, place of its V, whether it starts its share, the share.
@@ -963,7 +986,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&s_empty[b]);
         if (any_of_128(raise)) {
-          // New references: the largest weight so far counts as 2^4, the largest term of a sum as 1.
+          // New references: the largest weight so far counts as 2^11, the largest term of a sum as 1.
 #pragma unroll
           for (int i = 0; i < HG; ++i) {
             const float a = warp_max(x[i] + lv[i / GP]), c = warp_max(x[i]);
@@ -976,12 +999,12 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 top = *reinterpret_cast<const float2*>(red_s + (k * 16 + tid) * 2);
-              nm = fmaxf(nm, top.x - 4.f);
+              nm = fmaxf(nm, top.x - kTopWeight);
               nr = fmaxf(nr, top.y);
             }
             c_s[tid] = make_float2(nm == -INFINITY ? 1.f : ptx::ex2(was.z - nm), nr == -INFINITY ? 1.f : ptx::ex2(was.w - nr));
             const bool used = tid % GP < nh;
-            ref_s[tid] = make_float4(used ? nm + 8.f : INFINITY, used ? nr + 64.f : INFINITY, nm, nr);
+            ref_s[tid] = make_float4(used ? nm + kMostWeight : INFINITY, used ? nr + 64.f : INFINITY, nm, nr);
           }
           if (t0 != cur.tok0) wait(&p_empty[b ^ 1], ((it - 1) >> 1) & 1);  // P.V of the tile before: O^T is at rest
           ptx::named_barrier_sync(1, 128);
@@ -990,7 +1013,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           for (int i = 0; i < HG; ++i) l[i] *= c_s[i].y;
           if (t0 != cur.tok0) {
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
+            for (int k = 0; k < 4; ++k) {
               float o[GP];
               const uint32_t at = lane_addr + L::kOCol + k * HG + my_hp * GP;
               umma::ld_32x32b<GP>(at, o);
@@ -1018,14 +1041,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
               l[i] += ptx::ex2(x[i] - ref.y);
               wt[k] = ptx::ex2(x[i] + lv[hp] - (ref.x == -INFINITY ? 0.f : ref.x));
             }
-            const uint32_t hw = DT<__half>::pack2(wt[0], wt[1]);
-            const uint32_t c1 = q8::encode2h(hw), r1 = q8::sub2h(hw, q8::decode2h(c1));
-            const uint32_t c2 = q8::encode2h(r1), r2 = q8::sub2h(r1, q8::decode2h(c2));
-            const __half2 r3 = __hmul2(*reinterpret_cast<const __half2*>(&r2), __float2half2_rn(256.f));
-            const uint32_t c3 = q8::encode2h(*reinterpret_cast<const uint32_t*>(&r3));
-            const uint32_t cs[3] = {c1, c2, c3};
+            uint32_t cs[4];
+            split_weights(wt[0], wt[1], cs);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
+            for (int k = 0; k < 4; ++k) {
               // swz128(row, tid): the row's part of the swizzle is an exclusive or of constants
               const int row = k * HG + hp * GP + h;
               store_byte((pw ^ ((row & 7) << 4)) + row * 128, cs[k]);
@@ -1059,13 +1078,20 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       }
       wait(&p_empty[(it - 1) & 1], ((it - 1) >> 1) & 1);
       umma::fence_after_sync();
-      float o[GP], o1[GP], o2[GP];
+      float o[GP];
       {
+        float a[GP], c[GP];
         const uint32_t at = lane_addr + L::kOCol + my_hp * GP;
-        umma::ld_32x32b<GP>(at, o);
-        umma::ld_32x32b<GP>(at + HG, o1);
-        umma::ld_32x32b<GP>(at + 2 * HG, o2);
+        umma::ld_32x32b<GP>(at + 2 * HG, a);
+        umma::ld_32x32b<GP>(at + 3 * HG, c);
         umma::ld_wait();
+#pragma unroll
+        for (int h = 0; h < GP; ++h) c[h] += a[h];
+        umma::ld_32x32b<GP>(at, o);
+        umma::ld_32x32b<GP>(at + HG, a);
+        umma::ld_wait();
+#pragma unroll
+        for (int h = 0; h < GP; ++h) o[h] += fmaf(c[h], kLowPart, a[h]);
       }
       umma::fence_before_sync();
       __syncwarp();
@@ -1086,14 +1112,14 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (part) {
 #pragma unroll
         for (int h = 0; h < GP; ++h)
-          __stcg(part + (r0 + h) * D + dim, (fmaf(o2[h], kLowPart, o1[h]) + o[h]) * c_s[r0 + h].x);
+          __stcg(part + (r0 + h) * D + dim, o[h] * c_s[r0 + h].x);
         if (tid == 0) cut_s[n_cut & 1] = cur;
         ++n_cut;
       } else if (head0 < p.n_heads) {
         T* out = reinterpret_cast<T*>(p.out) + ((size_t)cur.b * p.n_heads + head0) * D + dim;
 #pragma unroll
         for (int h = 0; h < GP; ++h)
-          if (h < nh) out[(size_t)h * D] = DT<T>::from_f((fmaf(o2[h], kLowPart, o1[h]) + o[h]) * c_s[r0 + h].x);
+          if (h < nh) out[(size_t)h * D] = DT<T>::from_f(o[h] * c_s[r0 + h].x);
       }
     }
 

@@ -65,19 +65,19 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool ab_bf16, boo
          | ((uint32_t)(M >> 4) << 24);               // M / 16
 }
 
-// Instruction descriptor for kind::f8f6f4 with e4m3 operands and fp32 accumulation
-// (K = 32 per instruction).  a_mn_major: A stored M-contiguous.  B is K-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool a_mn_major) {
+// Instruction descriptor for kind::f8f6f4 with e4m3 operands (b_e5m2: B in e5m2) and fp32
+// accumulation (K = 32 per instruction).  a_mn_major: A stored M-contiguous.  B is K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool a_mn_major, bool b_e5m2 = false) {
   return (1u << 4)                                   // D format F32
          | (0u << 7)                                 // A format E4M3
-         | (0u << 10)                                // B format E4M3
+         | ((b_e5m2 ? 1u : 0u) << 10)                // B format E4M3 or E5M2
          | ((a_mn_major ? 1u : 0u) << 15)            // A major-ness
          | ((uint32_t)(N >> 3) << 17)                // N / 8
          | ((uint32_t)(M >> 4) << 24);               // M / 16
 }
 
 // ---- MMA ---------------------------------------------------------------------
-// D[tmem] (+)= A[smem] * B[smem], e4m3 operands; one thread issues.
+// D[tmem] (+)= A[smem] * B[smem], 8-bit operands; one thread issues.
 __device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
   asm volatile(
