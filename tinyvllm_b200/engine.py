@@ -246,6 +246,7 @@ class LLMEngine:
         self._prefill_pool = None
         self._prefill_stream = None
         self._graph_width = self.table_width or -(-2 * cfg.max_seq_len // block_size)
+        self._step_logprobs: Dict[int, SampledLogprobs] = {}   # of the tokens being sampled, by sequence
 
     # ------------------------------------------------------------------ API
     def add_request(self, prompt, sampling_params: Optional[SamplingParams] = None,
@@ -301,7 +302,7 @@ class LLMEngine:
         if prefill:
             first = self._prefill(prefill)
             for seq, tok in zip(prefill, first):
-                seq.append_token(tok)
+                self._append(seq, tok)
                 if self._check_finished(seq):
                     finished.append(seq.seq_id)
         for _ in range(self.num_scheduler_steps):
@@ -310,7 +311,7 @@ class LLMEngine:
             next_tokens = self._decode(decode)
             still = []
             for seq, tok in zip(decode, next_tokens):
-                seq.append_token(tok)
+                self._append(seq, tok)
                 if self._check_finished(seq):
                     finished.append(seq.seq_id)
                 else:
@@ -330,6 +331,14 @@ class LLMEngine:
                     del self.requests[rid]
                     break
         return outs
+
+    def _append(self, seq: Sequence, token: int) -> None:
+        """Takes a sampled token with its log probabilities: together, once the step's checks have passed, so
+        that a step that raised leaves neither."""
+        seq.append_token(token)
+        entry = self._step_logprobs.pop(seq.seq_id, None)
+        if seq.logprobs is not None:
+            seq.logprobs.append(entry)
 
     def _reason(self, seq: Sequence) -> str:
         return "eos" if seq.output_tokens[-1] == self.tokenizer.eos_id else "length"
@@ -351,8 +360,6 @@ class LLMEngine:
                 bm.slot_mapping(s.seq_id, 0, s.get_prompt_len())
                 bm.advance_position(s.seq_id, s.get_prompt_len())
                 first[s.seq_id] = tok
-                if s.logprobs is not None:
-                    s.logprobs.append(None)
         if live:
             for s, t in zip(live, self._prefill_live(live)):
                 first[s.seq_id] = t
@@ -446,7 +453,8 @@ class LLMEngine:
 
     def _add_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, seqs: List[Sequence]) -> None:
         """Log probabilities of this step's ``tokens`` (int32, one per row of ``logits``) for
-        the sequences that asked for them: one call over all rows, read back once."""
+        the sequences that asked for them, kept for ``_append``: one call over all rows, read back once."""
+        self._step_logprobs = {}
         want = [self.requests[s.request_id].sampling_params.logprobs for s in seqs]
         n = max((w for w in want if w is not None), default=None)
         if n is None:
@@ -457,7 +465,7 @@ class LLMEngine:
         for s, w, row in zip(seqs, want, host):
             if w is not None:
                 top = [(int(t), lp) for t, lp in zip(row[3:3 + w], row[3 + n:3 + n + w])]
-                s.logprobs.append(SampledLogprobs(int(row[0]), row[1], row[2], top))
+                self._step_logprobs[s.seq_id] = SampledLogprobs(int(row[0]), row[1], row[2], top)
 
 
 def generate_batch(engine: LLMEngine, prompts: List, sampling_params: Optional[SamplingParams] = None) -> List[str]:
