@@ -118,3 +118,24 @@ def test_a_given_first_token_has_one_empty_entry_after_a_time_out(checks, bad):
         assert len(entries) == len(got[i].tokens) == 4
         assert [x and x.token for x in entries] == ([None] if i == 0 else got[1].tokens[:1]) + got[i].tokens[1:]
     assert got[1].logprobs == want[1].logprobs
+
+
+@pytest.mark.parametrize("bad", [(1,), (1, 2)])
+def test_a_prefill_done_again_advances_given_sequences_once(checks, bad):
+    """The step that admits a request with resident K/V beside one to prefill runs out of time, and is done again."""
+    def make():
+        eng = _engine()
+        eng.add_prefilled_request([5, 6, 7], SamplingParams(max_tokens=4), first_token=11)
+        eng.add_request([3, 4], SamplingParams(max_tokens=4))
+        return eng
+
+    want, got = _both(checks, bad, make)
+    assert [got[i].tokens for i in (0, 1)] == [want[i].tokens for i in (0, 1)]
+    checks.bad, checks.n = bad, 0
+    eng = make()
+    for _ in bad:
+        with pytest.raises(TvkError):
+            eng.step()
+    eng.step()
+    bm = eng.block_manager
+    assert [bm.get_context_length(s) for s in sorted(eng.scheduler.running)] == [3, 2]

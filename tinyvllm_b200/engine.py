@@ -356,13 +356,15 @@ class LLMEngine:
             tok = self.requests[s.request_id].prefilled_first_token
             if tok is None:
                 live.append(s)
-            else:                      # K/V already resident: allocate and advance only
+            else:                      # K/V already resident: allocate, and advance below
                 bm.slot_mapping(s.seq_id, 0, s.get_prompt_len())
-                bm.advance_position(s.seq_id, s.get_prompt_len())
                 first[s.seq_id] = tok
         if live:
             for s, t in zip(live, self._prefill_live(live)):
                 first[s.seq_id] = t
+        for s in seqs:                 # after the prefill, which may raise: a step done again advances once
+            if self.requests[s.request_id].prefilled_first_token is not None:
+                bm.advance_position(s.seq_id, s.get_prompt_len())
         return [first[s.seq_id] for s in seqs]
 
     def _prefill_live(self, seqs: List[Sequence]) -> List[int]:
