@@ -139,3 +139,18 @@ def test_a_prefill_done_again_advances_given_sequences_once(checks, bad):
     eng.step()
     bm = eng.block_manager
     assert [bm.get_context_length(s) for s in sorted(eng.scheduler.running)] == [3, 2]
+
+
+@pytest.mark.parametrize("steps", [1, 3])
+@pytest.mark.parametrize("bad", [(3,), (4,), (3, 4), (6,)])
+def test_sequences_that_finished_before_a_time_out_end_there(checks, bad, steps):
+    """A sequence that reaches its length in a step whose later part raises gets no further token, and is reported."""
+    def make():
+        eng = _engine(num_scheduler_steps=steps, max_batch_size=2)
+        for i, n in enumerate([6, 1, 1, 2, 3]):
+            eng.add_request([3 + i, 4], SamplingParams(max_tokens=n, logprobs=0))
+        return eng
+
+    want, got = _both(checks, bad, make)
+    assert {i: o.tokens for i, o in got.items()} == {i: o.tokens for i, o in want.items()}
+    assert [len(got[i].logprobs) for i in range(5)] == [6, 1, 1, 2, 3]

@@ -246,6 +246,7 @@ class LLMEngine:
         self._prefill_pool = None
         self._prefill_stream = None
         self._graph_width = self.table_width or -(-2 * cfg.max_seq_len // block_size)
+        self._finished: List[int] = []     # sequences whose last token is there, until their step reports them
         self._step_logprobs: Dict[int, SampledLogprobs] = {}   # of the tokens being sampled, by sequence
 
     # ------------------------------------------------------------------ API
@@ -296,9 +297,9 @@ class LLMEngine:
         batch = self.scheduler.schedule()
         if not batch.scheduled_seqs:
             return []
-        finished: List[int] = []
+        finished = self._finished        # not empty only where the step before raised after they finished
         prefill = [s for s in batch.scheduled_seqs if s.get_output_len() == 0]
-        decode = [s for s in batch.scheduled_seqs if s.get_output_len() > 0]
+        decode = [s for s in batch.scheduled_seqs if s.get_output_len() > 0 and s.seq_id not in finished]
         if prefill:
             first = self._prefill(prefill)
             for seq, tok in zip(prefill, first):
@@ -318,6 +319,7 @@ class LLMEngine:
                     still.append(seq)
             decode = still
         self.scheduler.update(finished)
+        self._finished = []
         outs = []
         for sid in finished:
             for rid, req in list(self.requests.items()):
