@@ -46,6 +46,8 @@ class _Req:
     max_tokens: int
     tokens: List[int] = field(default_factory=list)
     finished: bool = False
+    # on the owner, where SamplingParams.logprobs asked for them: one entry per token so far
+    logprobs: Optional[List[Any]] = None
 
 
 class ShardedEngine:
@@ -56,6 +58,10 @@ class ShardedEngine:
     ``num_scheduler_steps``; the new tokens of a step are read from the
     engine's request table (``engine.requests[rid].sequence.output_tokens``)
     and its finished outputs.
+
+    ``requests[rid].tokens`` is every rank's; the log probabilities that
+    ``SamplingParams.logprobs`` asks for are not exchanged: ``requests[rid].logprobs`` is
+    the owner's, None elsewhere.
     """
 
     def __init__(self, engine: Any, rank: int, world_size: int, device: torch.device,
@@ -168,7 +174,9 @@ class ShardedEngine:
             seq = getattr(r, "sequence", None)
             if seq is not None:
                 new.extend((rid, int(t), 0) for t in seq.output_tokens[before.get(rid, 0):])
+                self.requests[rid].logprobs = getattr(seq, "logprobs", None)
         for o in finished_outs:
+            self.requests[o.request_id].logprobs = getattr(o, "logprobs", None)
             tail = list(o.tokens)[before.get(o.request_id, 0):]
             new.extend((o.request_id, int(t), int(j == len(tail) - 1)) for j, t in enumerate(tail))
         return new
