@@ -201,7 +201,8 @@ struct Sums {
 // c (t + d s) for a move of the reference by d, c = 2^d; 0 where c is (d s may overflow there).
 __device__ __forceinline__ float moved(float c, float d, float s, float t) { return c == 0.f ? 0.f : c * fmaf(d, s, t); }
 
-// New reference: m > a.m, or NaN (then everything becomes NaN, as it should).
+// New reference: m > a.m, or NaN (then everything becomes NaN, as it should, and stays it: a later step of
+// nothing but -inf must not look like a start).
 __device__ __forceinline__ void raise_max(Sums& a, float m) {
   if (a.m == -INFINITY) {  // nothing but -inf so far
     const float z = m != m ? m : 0.f;
@@ -212,7 +213,7 @@ __device__ __forceinline__ void raise_max(Sums& a, float m) {
     a.t = pack(moved(c, d, s.x, t.x), moved(c, d, s.y, t.y));
     a.s = mul2(a.s, pack(c, c));
   }
-  a.m = m;
+  a.m = max_nan(a.m, m);
 }
 
 // With any reference.  x - m is formed before the scaling to base 2, so rows that hold nothing
