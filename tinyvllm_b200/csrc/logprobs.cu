@@ -46,7 +46,7 @@ constexpr int kLpBuf = 2048;         // candidate keys kept in shared memory
 constexpr int kLpMaxK = 32;
 constexpr int kLpGroups = 64;        // groups of threads, or of keys, whose maxima give a threshold
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLpFloor = -30000.f;  // see add_step
+constexpr float kLpFloor = -30000.f, kLpCeiling = 1e38f;  // see add_step
 
 // fp32 values as unsigned integers of the same order: -0 counts as +0, every
 // NaN as one value above +inf.
@@ -230,12 +230,13 @@ __device__ __forceinline__ void add_pair(Sums& a, F2 x) {
 }
 
 // A step's vectors.  With an ordinary reference (almost always) 16-bit elements are floored two
-// at a time: what lies below -30000 weighs nothing beside it, and no product with -inf arises.
+// at a time: what lies below -30000 weighs nothing beside it, and no product with -inf arises (up to a
+// reference of 1e38: beyond, (x - m) log2 e may pass the fp32 range, which add_pair looks after).
 // The first n vectors; ALL: every one, without a branch between them.
 template <typename T, bool ALL>
 __device__ __forceinline__ void add_step(Sums& a, const uint4 (&u)[kLpUnroll], int n) {
   constexpr int N = 16 / sizeof(T);
-  if (sizeof(T) == 2 && a.m > kLpFloor + 1000.f && a.m < INFINITY) {
+  if (sizeof(T) == 2 && a.m > kLpFloor + 1000.f && a.m < kLpCeiling) {
     const F2 scale = pack(kLog2e, kLog2e), minus_m = pack(-a.m, -a.m);
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
