@@ -1,5 +1,5 @@
-"""Token log probabilities of rows with NaN before a masked span, and of logits near
-their type's largest value (GPU).  Bounds as derived at the head of test_logprobs.py."""
+"""Token log probabilities of rows with NaN before a masked span, of logits near their
+type's largest value, and of rows of ties (GPU).  Bounds as derived at the head of test_logprobs.py."""
 
 import numpy as np
 import pytest
@@ -54,3 +54,71 @@ def test_logits_near_the_largest_value(cuda, dtype, rows, V):
     for k in (0, 1):
         got = layers.token_logprobs(view, all_tok, k)
         _check(x, tok, k, layers.TokenLogprobs(*(t[at] for t in got)))
+
+
+def _time(fn, n=5):
+    fn()
+    best = float("inf")
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        fn()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("kind", ["constant", "descending", "masked"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_ties_are_not_pushed_again_step_after_step(cuda, dtype, kind):
+    """Once the K best are known exactly, nothing further of such rows is a candidate: the slow way through a full buffer is
+    taken once, not for the whole row.  A row is 31 (bf16) or 62 (fp32) full steps long."""
+    from tinyvllm_b200 import layers
+    rows, V, k = 296, 256000, 20
+    ordinary = torch.randn(rows, V, device=cuda).to(dtype)
+    tok = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    base = _time(lambda: layers.token_logprobs(ordinary, tok, k))
+    if kind == "constant":
+        x = torch.full((rows, V), 1.5, device=cuda, dtype=dtype)
+    elif kind == "descending":
+        x = (-torch.arange(V, device=cuda) * 2.0 ** -8).to(dtype).expand(rows, V).contiguous()
+    else:
+        x = torch.full((rows, V), -float("inf"), device=cuda, dtype=dtype)
+        x[:, 1000::20000] = 1.0
+    took = _time(lambda: layers.token_logprobs(x, tok, k))
+    print(f"{dtype} {kind}: {took * 1e3:.0f} us, ordinary {base * 1e3:.0f} us")
+    assert took <= 4 * base, f"{kind} rows take {took / base:.1f} times ordinary ones"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(300, 40000), (3, 200000)])
+def test_thresholds_of_full_buffers(cuda, dtype, rows, V):
+    """Rows that overflow the candidate buffer and then hold better, equal and fewer tokens; NaN at the row's first places."""
+    from tinyvllm_b200 import layers
+    nan, none = float("nan"), -float("inf")
+    x = torch.zeros(8, V, device=cuda)
+    x[0, V - 50:] = torch.arange(50, device=cuda) * 0.25          # the K best come last
+    x[1, ::3] = 0.5
+    x[2] = none
+    x[2, ::V // 7] = 1.0                                           # fewer tokens than alternatives
+    x[3, :] = nan
+    x[4, :2] = nan
+    x[5] = torch.arange(V, device=cuda) // 2000 * 0.125            # steps up: every threshold falls behind
+    x[6] = -(torch.arange(V, device=cuda) // 2000) * 0.125
+    x[7, 0], x[7, 9000:9020] = nan, 3.0
+    x = x.to(dtype)
+    tok = torch.arange(8, dtype=torch.int32, device=cuda) * 5
+    if rows == 3:
+        parts = [torch.arange(0, 3), torch.arange(3, 6), torch.arange(5, 8)]
+    else:
+        parts = [torch.arange(8)]
+    for k in (1, 2, 20, 32):
+        for part in parts:
+            view = torch.zeros(rows, V, device=cuda, dtype=dtype)
+            at = torch.linspace(0, rows - 1, len(part)).long().to(cuda)
+            p = part.to(cuda)
+            all_tok = torch.zeros(rows, dtype=torch.int32, device=cuda)
+            view[at], all_tok[at] = x[p], tok[p]
+            got = layers.token_logprobs(view, all_tok, k)
+            _check(x[p], tok[p], k, layers.TokenLogprobs(*(t[at] for t in got)))
