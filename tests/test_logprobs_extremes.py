@@ -122,3 +122,25 @@ def test_thresholds_of_full_buffers(cuda, dtype, rows, V):
             view[at], all_tok[at] = x[p], tok[p]
             got = layers.token_logprobs(view, all_tok, k)
             _check(x[p], tok[p], k, layers.TokenLogprobs(*(t[at] for t in got)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [300, 3])
+def test_ties_between_the_last_elements_and_later_ones(cuda, dtype, rows):
+    """The elements behind the last whole vector are looked at first: of equal ones in between, which come later, the smaller
+    index counts."""
+    from tinyvllm_b200 import layers
+    V = 160007
+    x = torch.zeros(4, V, device=cuda)
+    x[:, 5], x[:, V - 1] = 2.0, 1.0
+    x[1, 50000] = 1.0
+    x[2, V - 40], x[2, V - 2] = 1.0, 1.0
+    x[3, 100000:100300] = 1.0
+    x = x[:rows].to(dtype)
+    view = torch.zeros(rows, V, device=cuda, dtype=dtype)
+    at = torch.linspace(0, rows - 1, len(x)).long().to(cuda)
+    view[at] = x
+    tok = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    for k in (2, 3, 5):
+        got = layers.token_logprobs(view, tok, k)
+        _check(x, tok[:len(x)], k, layers.TokenLogprobs(*(t[at] for t in got)))

@@ -630,8 +630,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
       }
       keep_best(sh, K, 0, 0, &tau_key);
     }
-    // All that follows has larger indices than what is kept, so ties with the K-th best are no candidates.
-    if (tau_key) tau = next_larger<T>(value_of((uint32_t)(tau_key >> 32)));
+    if (tau_key) {
+      // All that follows has larger indices than the K-th best, so ties with that are no candidates; unless it is one of the
+      // elements behind the last whole vector.
+      tau = value_of((uint32_t)(tau_key >> 32));
+      if ((int)(0xffffffffu - (uint32_t)tau_key) < head + to * N) tau = next_larger<T>(tau);
+    }
   }
 
   // This CTA's sums: the largest reference first, then every thread's sums relative to it.
