@@ -332,11 +332,12 @@ __device__ __forceinline__ int block_count(LpShared<NT>& sh, int c) {
 
 // Keeps the K largest keys of the buffer (all of them if there are no more),
 // at its front in any order; keys of elements [drop_lo, drop_hi) are dropped
-// first.  Returns how many stay; *kth gets the smallest kept key (0 if
-// fewer than K), which is an element's and never below what it was.  Every thread of the CTA takes part.
-// Not inlined: the few calls would grow the loop around them ([2048, 128256] bf16 100.9 instead of 98.6 us).
+// first.  sh.count says how many stay.  Returns the smallest kept key (0 if fewer than
+// K), which is an element's and never below what it was.  Every thread of the CTA takes part.
+// Not inlined, and the threshold by value: its few calls otherwise cost the loop around them registers and code
+// ([2048, 128256] bf16 100.9 us inlined with the threshold through a pointer, 95.7 so; fp32 no difference).
 template <int NT>
-__device__ __noinline__ int keep_best(LpShared<NT>& sh, int K, int drop_lo, int drop_hi, unsigned long long* kth) {
+__device__ __noinline__ unsigned long long keep_best(LpShared<NT>& sh, int K, int drop_lo, int drop_hi) {
   __syncthreads();
   const int n = min(sh.count, kLpBuf);
   unsigned long long mine[(kLpBuf / NT)];
@@ -380,8 +381,7 @@ __device__ __noinline__ int keep_best(LpShared<NT>& sh, int K, int drop_lo, int 
   unsigned long long least = kept >= K ? ~0ull : 0ull;
   for (int i = 0; kept >= K && i < kept; ++i) least = min(least, sh.keys[i]);
   __syncthreads();  // all have read the count before anyone pushes again
-  *kth = least;
-  return kept;
+  return least;
 }
 
 __device__ __forceinline__ unsigned long long key_of(float x, int idx) {
@@ -464,7 +464,7 @@ __device__ uint32_t reached_by_k(LpShared<NT>& sh, int K) {
 
 // The K best keys of the buffer, in order, into sh.best; fewer if there are no more.
 template <int NT>
-__device__ void select_best(LpShared<NT>& sh, int K, unsigned long long* scratch_kth) {
+__device__ void select_best(LpShared<NT>& sh, int K) {
   const int tid = threadIdx.x;
   __syncthreads();
   int n = sh.count;
@@ -483,7 +483,10 @@ __device__ void select_best(LpShared<NT>& sh, int K, unsigned long long* scratch
       n = sh.count;
       few = n <= NT;  // many only where many are equal
     }
-    if (!few) n = keep_best(sh, K, 0, 0, scratch_kth);
+    if (!few) {
+      keep_best(sh, K, 0, 0);
+      n = sh.count;
+    }
   }
   if (tid < n) {
     const unsigned long long k = sh.keys[tid];
@@ -613,11 +616,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
       continue;
     }
     if (sh.count <= kLpBuf) {
-      keep_best(sh, K, 0, 0, &tau_key);
+      tau_key = keep_best(sh, K, 0, 0);
     } else {
       // Keys of these steps were lost: take the steps out and push them again, one
       // element a thread at a time, cutting back whenever the next push might overflow.
-      keep_best(sh, K, head + from * N, head + to * N, &tau_key);
+      tau_key = keep_best(sh, K, head + from * N, head + to * N);
       for (int base = from; base < to; base += NT) {
         const int i = base + tid;
         for (int e = 0; e < N; ++e) {
@@ -625,10 +628,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
           __syncthreads();
           const bool cut = sh.count > kLpBuf - NT;
           __syncthreads();
-          if (cut) keep_best(sh, K, 0, 0, &tau_key);
+          if (cut) tau_key = keep_best(sh, K, 0, 0);
         }
       }
-      keep_best(sh, K, 0, 0, &tau_key);
+      tau_key = keep_best(sh, K, 0, 0);
     }
     if (tau_key) {
       // All that follows has larger indices than the K-th best, so ties with that are no candidates; unless it is one of the
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
       sh.sums = RowSums{m, s, t};
     }
   }
-  if (K > 0) select_best(sh, K, &tau_key);
+  if (K > 0) select_best(sh, K);
   if (ctas > 1)
     cluster_sync();
   else
