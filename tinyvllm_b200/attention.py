@@ -23,14 +23,17 @@ _workspaces: Dict[Tuple[int, int, str], torch.Tensor] = {}
 
 def _workspace(device: torch.device, nbytes: int, kind: str = "decode") -> torch.Tensor:
     """Per-(device, stream, kernel family) scratch buffer, grown on demand and zeroed
-    when created (its first word is the kernels' time-out status)."""
+    when created (its first word is the kernels' time-out status, which a larger buffer
+    takes over)."""
     key = (device.index if device.index is not None else torch.cuda.current_device(),
            torch.cuda.current_stream(device).cuda_stream, kind)
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
+            grown = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            if ws is not None:
+                grown[:4].copy_(ws[:4])
+            ws = _workspaces[key] = grown
         return ws
 
 
@@ -41,7 +44,8 @@ def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Op
     """While the current stream records a CUDA graph: a workspace of that graph and stream
     alone, so that graphs recorded on one stream, and branches of one graph, may run at
     the same time.  Its header and last ``zero_tail`` bytes are zeroed by the graph itself
-    at every replay.  It lies in the graph's memory pool and lives as long as that; here
+    at every replay; where a call needs a larger one than those before it, that takes over
+    their status word.  It lies in the graph's memory pool and lives as long as that; here
     it is only kept until the stream's next recording.  None while nothing is recorded."""
     if not torch.cuda.is_current_stream_capturing():
         return None
@@ -54,8 +58,11 @@ def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Op
     with _ws_lock:
         of, ws = _capture_workspaces.get(key, (0, None))
         if of != capture.value or ws.numel() < nbytes:
+            before = ws if of == capture.value else None
             ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", index))
             ws[:256].zero_()
+            if before is not None:
+                ws[:4].copy_(before[:4])
             if zero_tail:
                 ws[nbytes - zero_tail:].zero_()
             _capture_workspaces[key] = (capture.value, ws)
