@@ -41,20 +41,23 @@ _capture_workspaces: Dict[tuple, Tuple[int, torch.Tensor]] = {}
 
 
 def _capture_workspace(index: int, nbytes: int, kind: str, zero_tail: int) -> Optional[torch.Tensor]:
-    """While the current stream records a CUDA graph: a workspace of that graph and stream
+    """While device ``index``'s current stream records a CUDA graph: a workspace of that graph and stream
     alone, so that graphs recorded on one stream, and branches of one graph, may run at
     the same time.  Its header and last ``zero_tail`` bytes are zeroed by the graph itself
     at every replay; where a call needs a larger one than those before it, that takes over
     their status word.  It lies in the graph's memory pool and lives as long as that; here
     it is only kept until the stream's next recording.  None while nothing is recorded."""
-    if not torch.cuda.is_current_stream_capturing():
+    if index == torch.cuda.current_device() and not torch.cuda.is_current_stream_capturing():
+        return None
+    stream = _lib.raw_stream(index)
+    if stream == 0:                      # a device's default stream cannot record
         return None
     capture = ctypes.c_ulonglong()
-    rc = _lib.lib().tvk_stream_capture_id(ctypes.byref(capture), _lib.raw_stream(index))
+    rc = _lib.lib().tvk_stream_capture_id(ctypes.byref(capture), stream)
     _lib.check(rc, "tvk_stream_capture_id")
-    if capture.value == 0:               # another device's stream is the one that records
+    if capture.value == 0:               # another device's stream records, or none does
         return None
-    key = (index, _lib.raw_stream(index), kind)
+    key = (index, stream, kind)
     with _ws_lock:
         of, ws = _capture_workspaces.get(key, (0, None))
         if of != capture.value or ws.numel() < nbytes:
