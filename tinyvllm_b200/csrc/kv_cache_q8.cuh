@@ -61,22 +61,6 @@ __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
 }
 
-// Asynchronous 16-byte copy global -> shared, and the thread's wait for all of its copies.
-__device__ __forceinline__ void copy16_async(uint4* dst, const uint4* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
-}
-// Zeros when !live (src is not read then).
-__device__ __forceinline__ void copy16_async_or_zeros(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// The thread's wait for all groups of copies but the newest N.
-template <int N>
-__device__ __forceinline__ void wait_copies_but() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // Two halves -> two e5m2 codes, nearest, ties to even.
 __device__ __forceinline__ uint32_t encode2h_e5m2(uint32_t h) {
   uint32_t r;

@@ -225,9 +225,9 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) write_kv_q8_kernel(
           const T* src = x + (size_t)row_of[rows[w.row]] * row_elems + w.c * 8;
           uint4* dst = stage + (i - lane) * kVecs;
 #pragma unroll
-          for (int k = 0; k < kVecs; ++k) q8::copy16_async(dst + k, reinterpret_cast<const uint4*>(src) + k);
+          for (int k = 0; k < kVecs; ++k) ptx::copy16_async(dst + k, reinterpret_cast<const uint4*>(src) + k);
         }
-        q8::wait_copies();
+        ptx::wait_copies();
       };
       float amax = 0.f;
       for (int from = 0; from < items; from += kItems) {

@@ -34,7 +34,6 @@
 // ones 70 and 63.
 #include <math.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "tvk_common.cuh"
@@ -388,13 +387,6 @@ __device__ __forceinline__ unsigned long long key_of(float x, int idx) {
   return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - (uint32_t)idx);
 }
 
-// Asynchronous 16-byte copy global -> shared, and the thread's wait for all groups of copies but the newest.
-__device__ __forceinline__ void copy16_async(uint4* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_copies_but_1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
@@ -525,9 +517,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
       const int i = base + k * NT + tid;
-      if (i < v1) copy16_async(ring + (half * kLpUnroll + k) * NT + tid, xv + (size_t)i * N);
+      if (i < v1) ptx::copy16_async(ring + (half * kLpUnroll + k) * NT + tid, xv + (size_t)i * N);
     }
-    commit_copies();
+    ptx::commit_copies();
   };
   int half = 0;
   if constexpr (kRing) fetch(0, v0);
@@ -564,7 +556,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LpP
       uint4 u[kLpUnroll];  // -inf where there is no vector
       if constexpr (kRing) {
         fetch(half ^ 1, base + kLpUnroll * NT);  // into the places read in the step before
-        wait_for_copies_but_1();
+        ptx::wait_copies_but<1>();
       }
 #pragma unroll
       for (int k = 0; k < kLpUnroll; ++k) {
@@ -716,15 +708,9 @@ template <typename T, int NT>
 cudaError_t launch_nt(const LpParams& p, int rows, int ctas, cudaStream_t stream) {
   constexpr int kRingBytes = NT == 256 ? 2 * kLpUnroll * NT * 16 : 0;
   auto kern = token_logprobs_kernel<T, NT>;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = tvk::allow_smem(kern, kRingBytes, allowed);
   if (e != cudaSuccess) return e;
-  static std::atomic<unsigned long long> attr_set{0};  // one bit per device
-  if (dev >= 64 || !(attr_set.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) attr_set.fetch_or(1ull << dev);
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * ctas);
   cfg.blockDim = NT;

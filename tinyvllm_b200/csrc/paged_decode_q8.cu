@@ -20,7 +20,6 @@
 // for the joins of many parts.)
 #include <math.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "kv_cache_q8.cuh"
@@ -33,7 +32,7 @@ constexpr int kSimtWhole = 2;        // its units of up to so many tiles are not
 constexpr int kTcTile = 128;         // the same for the tensor-core kernel: the rows of a matrix instruction
 constexpr int kTcWhole = 6;          // joining parts costs as much as 4 to 5 tiles in a row
 constexpr int kMaxGroup = 16;        // query heads per KV head
-constexpr int kSimtCtas = 592;       // four CTAs on each of 148 SMs (two at 16 query heads: the second half follows)
+constexpr int kSimtCtas = 592;       // four CTAs on each of 148 SMs (with 16 query heads two fit, and the others follow as those end)
 constexpr int kTcCtas = 296;         // two CTAs on each SM
 constexpr int kMaxPieces = kSimtCtas;
 constexpr int kUnitTiles = 2;        // what a unit's start and end count as on the work line
@@ -308,11 +307,11 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
         const int t = r + lane / kChunks;
         const size_t at = __shfl_sync(0xffffffffu, (unsigned long long)row, t);
         const bool live = __shfl_sync(0xffffffffu, blk, t) >= 0;
-        q8::copy16_async_or_zeros(ptx::smem_u32(codes[kv] + t * L::kPitch + lane % kChunks * 16), pool + at * D + lane % kChunks * 16, live);
+        ptx::copy16_async_or_zeros(ptx::smem_u32(codes[kv] + t * L::kPitch + lane % kChunks * 16), pool + at * D + lane % kChunks * 16, live);
       }
       const float* src = kv ? p.v_scale : p.k_scale;
       q8::copy4_async(ptx::smem_u32(scales + kv * kSimtWarpTile + lane), blk >= 0 ? src + (size_t)blk * Hkv + s.h : src, blk >= 0);
-      q8::commit_copies();
+      ptx::commit_copies();
     };
     float acc[GM][DV], m[GM], l[GM];
 #pragma unroll
@@ -330,7 +329,7 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
     }
     for (int t0 = first; t0 < s.tok1; t0 += step) {
       const int next = block_of(t0 + step);  // all -1 behind the end: the copies are zeros that nobody reads
-      q8::wait_copies_but<1>();
+      ptx::wait_copies_but<1>();
       __syncwarp();
       float x[GM];
 #pragma unroll
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
       __syncwarp();  // every lane has read K and its scale
       issue(0, t0 + step, next);
       float corr[GM];
-      q8::wait_copies_but<1>();
+      ptx::wait_copies_but<1>();
       const float sv = scales[kSimtWarpTile + lane];
 #pragma unroll
       for (int h = 0; h < GM; ++h) {
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(128, GM == 16 ? 2 : 4) paged_decode_q8_simt_ke
       issue(1, t0 + step, next);
     }
     // The warps' sums, relative to each warp's maxima, in place of its tiles.
-    q8::wait_copies();
+    ptx::wait_copies();
     __syncwarp();
     float* sums = reinterpret_cast<float*>(mine);  // [GM][D], then (maximum, sum) of every head
 #pragma unroll
@@ -1195,25 +1194,12 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   }
 }
 
-// Lets a kernel have its dynamic shared memory, once per device.  A, B: so that each kernel has its own record.
-template <int A, int B, typename K>
-int allow_smem(K kern, int bytes) {
-  int dev = 0;
-  TVK_CHECK_CUDA(cudaGetDevice(&dev));
-  static std::atomic<unsigned long long> set{0};  // one bit per device
-  if (dev >= 64 || !(set.load() >> dev & 1)) {
-    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev < 64) set.fetch_or(1ull << dev);
-  }
-  return TVK_OK;
-}
-
 template <int D, int GM>
 int launch_simt_gm(const Q8Params& p, cudaStream_t stream) {
   using L = SimtLayout<D, GM>;
   auto kern = paged_decode_q8_simt_kernel<D, GM>;
-  const int rc = allow_smem<D, GM>(kern, L::kBytes);
-  if (rc != TVK_OK) return rc;
+  static std::atomic<unsigned long long> allowed{0};
+  TVK_CHECK_CUDA(tvk::allow_smem(kern, L::kBytes, allowed));
   const long long most = (long long)p.batch * p.n_kv_heads * (tiles_of(p.max_ctx_tokens, kSimtTile) + kUnitTiles);
   const int grid = (int)(most < kSimtCtas ? most : kSimtCtas);
   TVK_CHECK_CUDA(tvk::launch_pdl(kern, grid, 128, L::kBytes, stream, p));
@@ -1260,13 +1246,8 @@ int launch_tc(const Q8Params& p, cudaStream_t stream) {
     }
   }
   auto kern = paged_decode_q8_tc_kernel<T, D, GP>;
-  int dev = 0;
-  TVK_CHECK_CUDA(cudaGetDevice(&dev));
-  static std::atomic<unsigned long long> attr_set{0};  // one bit per device
-  if (dev >= 64 || !(attr_set.load() >> dev & 1)) {
-    TVK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-    if (dev < 64) attr_set.fetch_or(1ull << dev);
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  TVK_CHECK_CUDA(tvk::allow_smem(kern, L::kBytes, allowed));
   const int units = (p.n_kv_heads + L::HP - 1) / L::HP * ((p.group + GP - 1) / GP);
   // Teams of up to 8 CTAs on neighbouring units of the same tokens: what they read lies side by side in
   // the pool, and they read it at about the same time.

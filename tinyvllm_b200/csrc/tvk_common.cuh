@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <atomic>
 #include <string>
 
 #include "../../include/tvk.h"
@@ -92,6 +93,18 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
 
+// Lets a kernel have its dynamic shared memory on the current device, once; `done`: the kernel's own record, a bit
+// per device.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+  return e;
+}
+
 }  // namespace tvk
 
 // ----------------------------------------------------------------------------
@@ -162,6 +175,22 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+
+// Asynchronous 16-byte copy global -> shared, and the thread's wait for all of its copies.
+__device__ __forceinline__ void copy16_async(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Zeros when !live (src is not read then).
+__device__ __forceinline__ void copy16_async_or_zeros(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// The thread's wait for all groups of copies but the newest N.
+template <int N>
+__device__ __forceinline__ void wait_copies_but() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Whether the phase with the given parity has completed; never suspends.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {

@@ -289,7 +289,6 @@ class Llama:
         h = layers.embedding(self.tok_embeddings, tokens)
         x = layers.rms_norm(h, self.layers[0].attention_norm, c.norm_eps)
         for i, L in enumerate(self.layers):
-            kc, vc = kv_cache.k_cache[i], kv_cache.v_cache[i]
             append_first = kv_order == "append_first"
             if append_first and not kv_cache.quantized:
                 q, k, v = self._qkv(L, x, positions, slots, kv_cache, i)
@@ -306,7 +305,7 @@ class Llama:
                 if kv_cache.quantized:
                     kv_cache.write_slots(i, k, v, slots)
                 else:
-                    late_kv = (k, v, slots, kc, vc)
+                    late_kv = (k, v, slots, kv_cache.k_cache[i], kv_cache.v_cache[i])
             nxt = self.layers[i + 1].attention_norm if i + 1 < c.n_layers else self.norm
             x = self._layer_ffn(L, h, attn, nxt, B, write_kv=late_kv)
         return torch.matmul(x, self.output)
