@@ -303,6 +303,8 @@ size_t tvk_paged_decode_q8_workspace_size(int batch, int n_kv_heads);
  * per KV head; any block size.  What lies behind a sequence's context is never
  * used, whatever it holds.  Scales are zero or positive; a block whose v_scale is negative
  * gives NaN.  q, k_cache, v_cache and workspace 16-byte aligned, out 4-byte; out does not overlap q.
+ * Scores, their maximum and the sum of weights are fp32; with 16-bit q a weight that multiplies V is off by at most
+ * 2^-15 of itself or 2^-36 of its row's largest, whichever is more.
  */
 int tvk_paged_decode_attention_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                   const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,

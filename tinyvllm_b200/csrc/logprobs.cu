@@ -12,26 +12,27 @@
 // maximum, some lane of a warp did so in most steps, which cost a third of the time).
 //
 // A row to itself (many rows) is a CTA's, whose vectors travel through shared memory a
-// step ahead: [2048, 128256] bf16 with one alternative takes 100 us so (5.2 TB/s, 0.80 of
-// the measured copy rate), with loads to registers 145 us, when a warp had nothing in flight
-// while it computed (and loads a step ahead in registers 203 us).  Without alternatives
-// 88 us; fp32 logits 157 and 162 us, 6.7 TB/s, all that memory gives.  What is left for bf16
+// step ahead: [2048, 128256] bf16 with one alternative takes 96 us so (5.5 TB/s, 0.84 of
+// the measured copy rate; 108 to 113 us called one by one), with loads to registers 145 us, when a warp had nothing in
+// flight while it computed (and loads a step ahead in registers 203 us).  Without alternatives
+// 86 us; fp32 logits 158 and 161 us, 6.6 TB/s, all that memory gives.  What is left for bf16
 // is the exponentials (58 us of the special-function unit) and the candidates' barriers.
 // With few rows a cluster of CTAs shares each, and their sums and K best are put
 // together by the first over distributed shared memory; they read once and are done, so
-// latencies bound them ([1, 128256] bf16 7.0 us, [64, 32000] fp16 with 20 alternatives 8.9 us).
+// latencies bound them ([1, 128256] bf16 7.0 us, [64, 32000] fp16 with 20 alternatives 8.8 us).
 //
 // The K best: from the maxima of 64 groups of threads over the first step
 // each CTA takes the K-th largest as a threshold, which K logits at least reach; one
 // below it is not among the K best.  What reaches it is pushed as a 64-bit key (ordered
 // value, inverted index) to shared memory; the same with groups of keys raises the threshold
 // after 4, 8 and 16 steps and every 16 from there, and leaves little more than the K best for
-// ranking at the end.  [2048, 128256] bf16 takes 127 us with K = 8, 157 with 20, 185 with 32
-// (with 32 groups and one raise 123, 183 and 429): pushing is what it costs.
+// ranking at the end.  [2048, 128256] bf16 takes 124 us with K = 8, 152 with 20, 181 with 32
+// (before the buffer's cut was taken out of the loop 127, 157 and 185; with 32 groups and one raise 123, 183 and
+// 429): pushing is what it costs.
 // Rows that keep pushing (sorted or constant logits) run into the buffer's
 // limit, are cut back to their K best and go on with an exact threshold, which what
-// comes later has to exceed: 296 constant rows of 256,000 take 102 (fp32) and 111 us (bf16), ordinary
-// ones 70 and 63.
+// comes later has to exceed: 296 constant rows of 256,000 take 100 (fp32) and 106 us (bf16), ordinary
+// ones 70 and 55.
 #include <math.h>
 
 #include <type_traits>
@@ -111,7 +112,7 @@ template <typename T> __device__ __forceinline__ T element(const uint4& u, int e
   }
 }
 
-// Bit e: element e is not below tau (NaN is not).  tau is -inf, NaN or an element's value, so that the 16-bit types hold it.
+// Bit e: element e is not below tau (NaN is not).  tau is -inf, NaN or a value of the type.
 template <typename T> __device__ __forceinline__ uint32_t not_below(const uint4& u, float tau) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   uint32_t bits = 0;

@@ -231,7 +231,7 @@ __device__ __forceinline__ float warp_max(float x) {
 // likewise.  Running maxima and sums are the warp's own; the four are put together at the end.
 //
 // Broadcast reads and products bound it: fp32, 16 sequences of 128-4096 tokens, 32/4 heads of 64 33 us, 8 with
-// 32/8 of 128 35 us (1.1 TB/s), 64 with 16/1 of 128 107 us, 4 sequences of 17-255 with 32/4 of 64 9.2 us.  (Codes decoded
+// 32/8 of 128 35 us (1.1 TB/s), 64 with 16/1 of 128 107-114 us, 4 sequences of 17-255 with 32/4 of 64 9.2 us.  (Codes decoded
 // to floats in shared memory by the whole CTA, a head per warp, took 60, 79, 174 and 14.5 us.)
 // -----------------------------------------------------------------------------
 constexpr int kSimtWarpTile = 32;
@@ -1267,7 +1267,8 @@ int launch_tc(const Q8Params& p, cudaStream_t stream) {
 // Calls that would leave most CTAs idle take units of 4 all the same: their tiles take half the
 // time, and the second reading of K and V comes from L2.  That is, of 4-head units either at
 // most 64 (32/4 heads of 64: one sequence of 512 tokens 12.9 -> 9.9 us, 8 of 8,192 22.5 -> 20.9),
-// or no more than there are CTAs, none of them cut (64 sequences of 40-640: 17.8 -> 15.5).
+// or no more than there are CTAs, none of them cut as far as the tables' width tells (64 sequences of 40-640 with tables
+// of 40 blocks: 17.8 -> 15.9; an engine's 64 blocks may hold longer contexts, and such calls take units of 8).
 // 32 sequences of 1,024 or 2,048 lose by it (17.4 -> 18.5, 20.6 -> 22.4).
 template <typename T>
 int launch_16bit(const Q8Params& p, int head_dim, cudaStream_t stream) {
