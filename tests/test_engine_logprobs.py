@@ -154,3 +154,16 @@ def test_sequences_that_finished_before_a_time_out_end_there(checks, bad, steps)
     want, got = _both(checks, bad, make)
     assert {i: o.tokens for i, o in got.items()} == {i: o.tokens for i, o in want.items()}
     assert [len(got[i].logprobs) for i in range(5)] == [6, 1, 1, 2, 3]
+
+
+def test_a_finished_sequence_that_is_aborted_before_its_step_is_done_again_is_not_reported(checks):
+    eng = _engine(max_batch_size=2)
+    a = eng.add_request([3, 4], SamplingParams(max_tokens=6))
+    eng.step()
+    b = eng.add_request([5, 4], SamplingParams(max_tokens=1))
+    checks.bad = (checks.n + 2,)                 # b's prefill is fine and ends it; the decode step behind it is not
+    with pytest.raises(TvkError):
+        eng.step()
+    assert eng.abort_request(b)
+    got = _run(eng)
+    assert list(got) == [a] and len(got[a].tokens) == 6

@@ -298,7 +298,8 @@ class LLMEngine:
         batch = self.scheduler.schedule()
         if not batch.scheduled_seqs:
             return []
-        finished = self._finished        # not empty only where the step before raised after they finished
+        # not empty only where the step before raised after they finished (some may have been aborted since)
+        finished = self._finished = [i for i in self._finished if i in self.scheduler.running]
         prefill = [s for s in batch.scheduled_seqs if s.get_output_len() == 0]
         decode = [s for s in batch.scheduled_seqs if s.get_output_len() > 0 and s.seq_id not in finished]
         if prefill:
